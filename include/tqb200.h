@@ -214,6 +214,108 @@ int tqb200_dev_matvec_gptq(const uint8_t *w, int has_g_idx, const float *x, floa
 int tqb200_matvec_f32(const float *w, const float *x, float *y, int out_dim, int in_dim);
 int tqb200_matvec_f16(const uint16_t *w, const float *x, float *y, int out_dim, int in_dim);
 
+/* ------------------------------------------------ many requests over a paged KV cache
+ * No reference counterpart (the reference and tqb200_engine decode one request over one
+ * contiguous cache).  For hosts that keep activations on the GPU and serve many sequences:
+ * per layer, tqb200_dev_paged_append (query/key norms, RoPE, cache write) and then
+ * tqb200_dev_paged_attention.  All pointers in this section are DEVICE pointers of the
+ * current device (another device's, or a host pointer, is TQB200_ERR_INVALID_ARG); calls are
+ * ordered on `stream`, allocate nothing, never synchronise, and may be captured in a CUDA
+ * graph (sequence lengths and page tables are read on the device at every replay).
+ *
+ * Element types of activations (q, k, v, out) and of the cache.  The cache's type is the
+ * activations' own, or TQB200_EL_F16 beside TQB200_EL_F32 activations; sums, norms and
+ * softmax statistics are fp32 or wider, and results are rounded once, to nearest even
+ * (fp16 subnormals kept: tqb200_engine's fp16 cache flushes |x| < 2^-24 as the reference
+ * does). */
+enum { TQB200_EL_F32 = 0, TQB200_EL_F16 = 1, TQB200_EL_BF16 = 2 };
+
+/* One layer's cache: element (page p, KV head h, slot j, dimension d) of k and of v at
+ * p * page_stride + h * head_stride + j * slot_stride + d (strides in elements, every one
+ * at least head_dim: [page][head][slot][dim] and [page][slot][head][dim] are both covered).
+ * head_dim: a multiple of 8 up to 256; head_dim 64 and 128 with 16-byte aligned rows take
+ * the tensor-core kernels. */
+typedef struct tqb200_paged_cache {
+    void *k, *v;
+    int type;          /* TQB200_EL_* */
+    int n_pages;
+    int page_size;     /* slots per page, any size >= 1 */
+    int n_kv_heads;
+    int head_dim;
+    long long page_stride, head_stride, slot_stride;
+} tqb200_paged_cache;
+
+/* The sequences of one call.  Sequence s has the token rows q_start[s] .. q_start[s+1]-1 of
+ * q, k, v and out as its newest positions, kv_len[s] positions in the cache with these
+ * included: its row i stands at position kv_len[s] - (q_start[s+1] - q_start[s]) + i.
+ * Position x lives in slot x % page_size of page page_table[s * table_stride + x / page_size];
+ * entries past the sequence's last page are never read.  Rows at and behind q_start[n_seqs]
+ * (a padded batch) are left as they are.  A sequence whose numbers do not fit (q_start
+ * decreasing or past n_tokens, more than max_q_len rows, kv_len negative or past
+ * table_stride pages) is skipped and TQB200_PAGED_BAD_SEQ recorded; a page index outside
+ * [0, n_pages) is neither read nor written, its positions count as masked, and
+ * TQB200_PAGED_BAD_PAGE is recorded. */
+typedef struct tqb200_paged_batch {
+    const int *q_start;     /* [n_seqs + 1], not decreasing */
+    const int *kv_len;      /* [n_seqs] */
+    const int *page_table;  /* [n_seqs][table_stride] */
+    int n_seqs;
+    int table_stride;       /* page indices per sequence */
+    int n_tokens;           /* rows of q, k, v and out */
+    int max_q_len;          /* the most rows that one sequence has */
+} tqb200_paged_batch;
+
+/* Codes that the kernels store to the optional device word `status` (left alone when the
+ * call finds nothing wrong; clear it beforehand). */
+enum {
+    TQB200_PAGED_TIMEOUT = 1,   /* a bounded wait inside the kernel ran out */
+    TQB200_PAGED_BAD_PAGE = 7,
+    TQB200_PAGED_BAD_SEQ = 8
+};
+
+/* Per-head RMSNorm of q and k (weights [head_dim] fp32, shared by the heads; NULL: none) and
+ * rotate-half RoPE over the first rotary_dim dimensions (0: none), in one pass:
+ *   y = x * (mean(x^2) + eps)^-1/2 * w,  then for i < rotary_dim / 2
+ *   (y_i, y_{i+rd/2}) turned by positions[t] * theta^(-2i/rotary_dim),
+ * the angle computed in double.  Token t's head h at q + t * q_stride + h * head_dim (strides
+ * in elements, so the rows may lie inside a fused q/k/v projection's output); q_out == q with
+ * equal strides works in place (any other overlap is undefined), likewise k; q or k NULL with
+ * 0 heads skips that side.  positions [n_tokens] (any int, negative ones included); may be
+ * NULL when rotary_dim is 0. */
+int tqb200_dev_qk_norm_rope(const void *q, const void *k, void *q_out, void *k_out, int type,
+                            int n_tokens, int n_heads, int n_kv_heads, int head_dim,
+                            int rotary_dim, long long q_stride, long long k_stride,
+                            long long q_out_stride, long long k_out_stride, const float *q_norm,
+                            const float *k_norm, float eps, float theta, const int *positions,
+                            void *stream);
+
+/* The same norms and rotation of every sequence's new rows, q to q_out (q NULL, n_heads 0: no
+ * queries) and k and v into the cache's pages, in one launch.  The rotation uses
+ * positions[row], or the row's cache position when positions is NULL.  Rows whose cache
+ * position is negative (kv_len below the sequence's new rows) are not stored.  Two rows that
+ * map to one slot (a page listed twice) race: either may end up there. */
+int tqb200_dev_paged_append(const void *q, const void *k, const void *v, void *q_out, int type,
+                            int n_heads, int rotary_dim, long long q_stride, long long k_stride,
+                            long long v_stride, long long q_out_stride, const float *q_norm,
+                            const float *k_norm, float eps, float theta, const int *positions,
+                            const tqb200_paged_cache *cache, const tqb200_paged_batch *batch,
+                            int *status, void *stream);
+
+/* Causal attention of every sequence's new rows over its cached positions (the new rows'
+ * own keys and values appended before):
+ *   out[row, h] = sum_{x <= p} softmax_x(scale * q[row, h] . K[x, h / (n_heads / n_kv_heads)]) V[x, ...]
+ * with p the row's position.  A row that sees no position (p < 0, or all its pages bad) gets
+ * zeros.  out may not overlap q.  The workspace holds
+ * tqb200_paged_attention_workspace_bytes() bytes, 16-byte aligned, zero before its first
+ * call; every call leaves it ready for the next.  One workspace serves any calls that do
+ * not overlap on the GPU (captured graphs included); calls that may overlap need one each. */
+size_t tqb200_paged_attention_workspace_bytes(const tqb200_paged_cache *cache,
+                                              const tqb200_paged_batch *batch, int n_heads);
+int tqb200_dev_paged_attention(const void *q, void *out, int type, int n_heads, long long q_stride,
+                               long long out_stride, float scale, const tqb200_paged_cache *cache,
+                               const tqb200_paged_batch *batch, void *workspace,
+                               size_t workspace_bytes, int *status, void *stream);
+
 /* -------------------------------------------------- whole-step decode engine
  * Replaces the GPU decode registry entry (GpuDecodeCreateFn / StepFn / ResetFn /
  * DestroyFn / LogitsFn, kernels/dispatch.h:353-378; the reference's engine is

@@ -1,0 +1,110 @@
+// paged_attention.cu — causal attention of new rows over a paged KV cache: the kernel for any
+// shape, and the choice of kernel, sm_100a.
+//
+//   out[t, h] = sum_{x <= p} e^(scale q.K[x] - M) V[x] / sum_{x <= p} e^(scale q.K[x] - M),
+// p the row's position, M any bound of the scores (the running maximum).
+#include <algorithm>
+#include <cfloat>
+
+#include "paged.cuh"
+
+namespace tqb200 {
+namespace {
+
+constexpr int kAnyThreads = 128;
+constexpr float kLog2e = 1.4426950408889634f;
+
+// One warp's pass over positions [x0, x1) for one row (its p >= x1 - 1): the running maximum
+// of the scaled scores (base 2), the sum and, in lane l, elements l, l + 32, ... of the
+// weighted values.  Every element type, head_dim up to 256 and alignment; positions on pages
+// outside the cache are passed over.
+template <typename T, typename C>
+__device__ void row_pass(const PagedAttnArgs &A, const T *q, int seq, int kv_head, int x0, int x1,
+                         float &m, float &l, float (&o)[8]) {
+    const int lane = threadIdx.x & 31, D = A.head_dim;
+    float qv[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        qv[j] = lane + 32 * j < D ? el_to_f<T>(q[lane + 32 * j]) : 0.0f;
+        o[j] = 0.0f;
+    }
+    m = -INFINITY;
+    l = 0.0f;
+    const float c = A.scale * kLog2e;
+    const int *row = A.b.table + (long long)seq * A.b.table_stride;
+    int bad = 0;
+    for (int x = x0; x < x1; ++x) {
+        const long long at = A.kv.offset(row, x, kv_head, &bad);
+        if (at < 0) continue;  // warp-uniform
+        const C *k = (const C *)A.kv.k + at, *v = (const C *)A.kv.v + at;
+        float s = 0.0f, vv[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const bool in = lane + 32 * j < D;
+            s = fmaf(qv[j], in ? el_to_f<C>(k[lane + 32 * j]) : 0.0f, s);
+            vv[j] = in ? el_to_f<C>(v[lane + 32 * j]) : 0.0f;
+        }
+        s = warp_sum(s) * c;
+        const float mn = fmaxf(m, s);
+        const float base = mn == -INFINITY ? 0.0f : mn;
+        const float f = exp2f(m - base), p = exp2f(s - base);
+        m = mn;
+        l = fmaf(l, f, p);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] = fmaf(o[j], f, p * vv[j]);
+    }
+    if (bad && lane == 0) report(A.status, TQB200_PAGED_BAD_PAGE);
+}
+
+// One warp per (row, head).
+template <typename T, typename C>
+__global__ void __launch_bounds__(kAnyThreads) paged_attn_any_kernel(const __grid_constant__ PagedAttnArgs A) {
+    const long long gw = (long long)blockIdx.x * (kAnyThreads / 32) + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    const long long tok_ll = gw / A.n_heads;
+    if (tok_ll >= A.b.n_tokens) return;
+    const int tok = (int)tok_ll, head = (int)(gw - tok_ll * A.n_heads);
+    const int s = seq_of_row(A.b, tok);
+    const SeqInfo q = seq_info(A.b, s);
+    if (!q.ok) {
+        if (lane == 0) report(A.status, TQB200_PAGED_BAD_SEQ);
+        return;
+    }
+    if (tok < q.q0 || tok >= q.q0 + q.n) return;
+    const int pos = q.len - q.n + (tok - q.q0);
+    float m, l, o[8];
+    row_pass<T, C>(A, (const T *)A.q + tok * A.q_stride + (long long)head * A.head_dim, s,
+                   head / (A.n_heads / A.n_kv_heads), 0, pos + 1, m, l, o);
+    T *out = (T *)A.out + tok * A.out_stride + (long long)head * A.head_dim;
+    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        if (lane + 32 * j < A.head_dim) out[lane + 32 * j] = el_from_f<T>(o[j] * inv);
+}
+
+template <typename T, typename C>
+int launch_any(const PagedAttnArgs &a, cudaStream_t st) {
+    const long long blocks = ((long long)a.b.n_tokens * a.n_heads + kAnyThreads / 32 - 1) / (kAnyThreads / 32);
+    TQ_CHECK_ARG(blocks < (1LL << 31), "paged_attention: %d tokens of %d heads", a.b.n_tokens, a.n_heads);
+    paged_attn_any_kernel<T, C><<<(unsigned)blocks, kAnyThreads, 0, st>>>(a);
+    TQ_CUDA_TRY(cudaGetLastError());
+    return TQB200_OK;
+}
+
+}  // namespace
+
+size_t paged_attention_work_bytes(int n_seqs, int n_tokens, int max_q_len, int n_heads,
+                                  int n_kv_heads, int head_dim) {
+    (void)n_seqs, (void)n_tokens, (void)max_q_len, (void)n_heads, (void)n_kv_heads, (void)head_dim;
+    return 16;
+}
+
+int launch_paged_attention(const PagedAttnArgs &a, cudaStream_t st) {
+    if (a.b.n_tokens == 0 || a.b.n_seqs == 0) return TQB200_OK;
+    if (a.type == TQB200_EL_F32)
+        return a.cache_type == TQB200_EL_F32 ? launch_any<float, float>(a, st) : launch_any<float, __half>(a, st);
+    if (a.type == TQB200_EL_F16) return launch_any<__half, __half>(a, st);
+    return launch_any<__nv_bfloat16, __nv_bfloat16>(a, st);
+}
+
+}  // namespace tqb200

@@ -34,6 +34,27 @@ class TQB200Error(RuntimeError):
         self.status = status
 
 
+EL_F32, EL_F16, EL_BF16 = 0, 1, 2  # TQB200_EL_*: element types of the paged-cache operators
+PAGED_TIMEOUT, PAGED_BAD_PAGE, PAGED_BAD_SEQ = 1, 7, 8  # codes of their status word
+
+
+class PagedCache(C.Structure):
+    """tqb200_paged_cache: one layer's paged K/V (device addresses, strides in elements)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("type", C.c_int), ("n_pages", C.c_int),
+                ("page_size", C.c_int), ("n_kv_heads", C.c_int), ("head_dim", C.c_int),
+                ("page_stride", C.c_longlong), ("head_stride", C.c_longlong),
+                ("slot_stride", C.c_longlong)]
+
+
+class PagedBatch(C.Structure):
+    """tqb200_paged_batch: the sequences of a call (device addresses of int32 arrays)."""
+    _fields_ = [("q_start", C.c_void_p), ("kv_len", C.c_void_p), ("page_table", C.c_void_p),
+                ("n_seqs", C.c_int), ("table_stride", C.c_int), ("n_tokens", C.c_int),
+                ("max_q_len", C.c_int)]
+
+
+_ll, _pc, _pb = C.c_longlong, C.POINTER(PagedCache), C.POINTER(PagedBatch)
+
 # name -> (argtypes, restype); every symbol include/tqb200.h declares appears here
 PROTOTYPES = {
     "tqb200_version": ([], _i),
@@ -98,6 +119,13 @@ PROTOTYPES = {
     "tqb200_dev_matvec_gptq": ([_vp, _i, _vp, _vp, _i, _i, _i, _vp], _i),
     "tqb200_matvec_f32": ([_f, _f, _f, _i, _i], _i),
     "tqb200_matvec_f16": ([_u16, _f, _f, _i, _i], _i),
+    "tqb200_dev_qk_norm_rope": ([_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _ll, _ll, _ll, _ll, _vp,
+                                 _vp, _fl, _fl, _vp, _vp], _i),
+    "tqb200_dev_paged_append": ([_vp, _vp, _vp, _vp, _i, _i, _i, _ll, _ll, _ll, _ll, _vp, _vp, _fl, _fl,
+                                 _vp, _pc, _pb, _vp, _vp], _i),
+    "tqb200_paged_attention_workspace_bytes": ([_pc, _pb, _i], C.c_size_t),
+    "tqb200_dev_paged_attention": ([_vp, _vp, _i, _i, _ll, _ll, _fl, _pc, _pb, _vp, C.c_size_t, _vp,
+                                    _vp], _i),
     "tqb200_engine_timeline": ([_vp, _i, _d, _d, _i32, C.POINTER(_i), C.POINTER(C.c_double)], _i),
     "tqb200_engine_timeline_launches": ([_vp, _i, _i, _i32, _d, C.POINTER(_i)], _i),
 }
@@ -216,6 +244,41 @@ def dev_matvec_i4_sym(w_ptr: int, x_ptr: int, y_ptr: int, out_dim: int, in_dim: 
 
 def dev_dequant_i4(w_ptr: int, rows: int, dim: int, group_size: int, out_ptr: int, stream=None):
     _check(load().tqb200_dev_dequant_i4(w_ptr, rows, dim, group_size, out_ptr, _stream(stream)))
+
+
+# ---------------------------------------------------------------- paged KV cache
+# Device addresses throughout; the arguments are those of include/tqb200.h.
+def dev_qk_norm_rope(q_ptr, k_ptr, q_out_ptr, k_out_ptr, el_type: int, n_tokens: int, n_heads: int,
+                     n_kv_heads: int, head_dim: int, rotary_dim: int, q_stride: int, k_stride: int,
+                     q_out_stride: int, k_out_stride: int, q_norm_ptr, k_norm_ptr, eps: float,
+                     theta: float, positions_ptr, stream=None):
+    _check(load().tqb200_dev_qk_norm_rope(q_ptr, k_ptr, q_out_ptr, k_out_ptr, el_type, n_tokens,
+                                          n_heads, n_kv_heads, head_dim, rotary_dim, q_stride,
+                                          k_stride, q_out_stride, k_out_stride, q_norm_ptr,
+                                          k_norm_ptr, eps, theta, positions_ptr, _stream(stream)))
+
+
+def dev_paged_append(q_ptr, k_ptr, v_ptr, q_out_ptr, el_type: int, n_heads: int, rotary_dim: int,
+                     q_stride: int, k_stride: int, v_stride: int, q_out_stride: int, q_norm_ptr,
+                     k_norm_ptr, eps: float, theta: float, positions_ptr, cache: PagedCache,
+                     batch: PagedBatch, status_ptr=None, stream=None):
+    _check(load().tqb200_dev_paged_append(q_ptr, k_ptr, v_ptr, q_out_ptr, el_type, n_heads,
+                                          rotary_dim, q_stride, k_stride, v_stride, q_out_stride,
+                                          q_norm_ptr, k_norm_ptr, eps, theta, positions_ptr, cache,
+                                          batch, status_ptr, _stream(stream)))
+
+
+def paged_attention_workspace_bytes(cache: PagedCache, batch: PagedBatch, n_heads: int) -> int:
+    """Bytes of the zeroed workspace that dev_paged_attention needs (0: arguments it refuses)."""
+    return load().tqb200_paged_attention_workspace_bytes(cache, batch, n_heads)
+
+
+def dev_paged_attention(q_ptr, out_ptr, el_type: int, n_heads: int, q_stride: int, out_stride: int,
+                        scale: float, cache: PagedCache, batch: PagedBatch, workspace_ptr,
+                        workspace_bytes: int, status_ptr=None, stream=None):
+    _check(load().tqb200_dev_paged_attention(q_ptr, out_ptr, el_type, n_heads, q_stride, out_stride,
+                                             scale, cache, batch, workspace_ptr, workspace_bytes,
+                                             status_ptr, _stream(stream)))
 
 
 # ---------------------------------------------------------------- VQ2 + BiIP
