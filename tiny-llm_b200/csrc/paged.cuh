@@ -188,10 +188,76 @@ struct PagedAttnArgs {
     int *status;
 };
 
+// ---------------------------------------------------------------- attention, shared
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// One warp's pass over positions [x0, x1) for one row (its p >= x1 - 1): the running maximum
+// of the scaled scores (base 2), the sum and, in lane l, elements l, l + 32, ... of the
+// weighted values.  Every element type, head_dim up to 256 and alignment; positions on pages
+// outside the cache are passed over.
+template <typename T, typename C>
+__device__ __noinline__ void row_pass(const PagedAttnArgs &A, const T *q, int seq, int kv_head, int x0, int x1,
+                         float &m, float &l, float (&o)[8]) {
+    const int lane = threadIdx.x & 31, D = A.head_dim;
+    float qv[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        qv[j] = lane + 32 * j < D ? el_to_f<T>(q[lane + 32 * j]) : 0.0f;
+        o[j] = 0.0f;
+    }
+    m = -INFINITY;
+    l = 0.0f;
+    const float c = A.scale * kLog2e;
+    const int *row = A.b.table + (long long)seq * A.b.table_stride;
+    int bad = 0;
+    for (int x = x0; x < x1; ++x) {
+        const long long at = A.kv.offset(row, x, kv_head, &bad);
+        if (at < 0) continue;  // warp-uniform
+        const C *k = (const C *)A.kv.k + at, *v = (const C *)A.kv.v + at;
+        float s = 0.0f, vv[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const bool in = lane + 32 * j < D;
+            s = fmaf(qv[j], in ? el_to_f<C>(k[lane + 32 * j]) : 0.0f, s);
+            vv[j] = in ? el_to_f<C>(v[lane + 32 * j]) : 0.0f;
+        }
+        s = warp_sum(s) * c;
+        const float mn = fmaxf(m, s);
+        const float base = mn == -INFINITY ? 0.0f : mn;
+        const float f = exp2f(m - base), p = exp2f(s - base);
+        m = mn;
+        l = fmaf(l, f, p);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] = fmaf(o[j], f, p * vv[j]);
+    }
+    if (bad && lane == 0) report(A.status, TQB200_PAGED_BAD_PAGE);
+}
+
+// ---------------------------------------------------------------- split attention
+// The work of a call is one line of tiles: for every sequence with rows, for every KV head,
+// (for every block of query rows,) the tiles of positions it reads.  CTA c takes tiles
+// [c quota, (c+1) quota), so every CTA reads equally many whatever the lengths are; the parts
+// of a (sequence, head, rows) item that lies in several CTAs are joined by the last of them
+// to arrive, in the order of the line (the result does not depend on who is last).  The item's
+// first CTA names its ticket; a CTA leaves at most two parts: that of the item it begins in
+// the middle of (slot 2c) and that of the item it ends in the middle of (slot 2c + 1).
+constexpr int kSplitMaxCtas = 1024;
+constexpr size_t kSplitTicketBytes = kSplitMaxCtas * 4;  // head of the workspace, zero between calls
+
 int launch_qk_norm_rope(const RopeArgs &a, cudaStream_t st);
 int launch_paged_append(const RopeArgs &a, const PagedView &kv, int cache_type, const BatchView &b,
                         int *status, cudaStream_t st);
 int launch_paged_attention(const PagedAttnArgs &a, cudaStream_t st);
+// At most 16 query rows per KV head, head_dim 64 or 128, 16-byte aligned rows.
+int launch_paged_decode(const PagedAttnArgs &a, int rows, cudaStream_t st);
+size_t paged_decode_work_bytes(int rows, int head_dim);
+constexpr int kDecodeRows = 16;
 size_t paged_attention_work_bytes(int n_seqs, int n_tokens, int max_q_len, int n_heads,
                                   int n_kv_heads, int head_dim);
 

@@ -12,49 +12,6 @@ namespace tqb200 {
 namespace {
 
 constexpr int kAnyThreads = 128;
-constexpr float kLog2e = 1.4426950408889634f;
-
-// One warp's pass over positions [x0, x1) for one row (its p >= x1 - 1): the running maximum
-// of the scaled scores (base 2), the sum and, in lane l, elements l, l + 32, ... of the
-// weighted values.  Every element type, head_dim up to 256 and alignment; positions on pages
-// outside the cache are passed over.
-template <typename T, typename C>
-__device__ void row_pass(const PagedAttnArgs &A, const T *q, int seq, int kv_head, int x0, int x1,
-                         float &m, float &l, float (&o)[8]) {
-    const int lane = threadIdx.x & 31, D = A.head_dim;
-    float qv[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        qv[j] = lane + 32 * j < D ? el_to_f<T>(q[lane + 32 * j]) : 0.0f;
-        o[j] = 0.0f;
-    }
-    m = -INFINITY;
-    l = 0.0f;
-    const float c = A.scale * kLog2e;
-    const int *row = A.b.table + (long long)seq * A.b.table_stride;
-    int bad = 0;
-    for (int x = x0; x < x1; ++x) {
-        const long long at = A.kv.offset(row, x, kv_head, &bad);
-        if (at < 0) continue;  // warp-uniform
-        const C *k = (const C *)A.kv.k + at, *v = (const C *)A.kv.v + at;
-        float s = 0.0f, vv[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const bool in = lane + 32 * j < D;
-            s = fmaf(qv[j], in ? el_to_f<C>(k[lane + 32 * j]) : 0.0f, s);
-            vv[j] = in ? el_to_f<C>(v[lane + 32 * j]) : 0.0f;
-        }
-        s = warp_sum(s) * c;
-        const float mn = fmaxf(m, s);
-        const float base = mn == -INFINITY ? 0.0f : mn;
-        const float f = exp2f(m - base), p = exp2f(s - base);
-        m = mn;
-        l = fmaf(l, f, p);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = fmaf(o[j], f, p * vv[j]);
-    }
-    if (bad && lane == 0) report(A.status, TQB200_PAGED_BAD_PAGE);
-}
 
 // One warp per (row, head).
 template <typename T, typename C>
@@ -95,12 +52,19 @@ int launch_any(const PagedAttnArgs &a, cudaStream_t st) {
 
 size_t paged_attention_work_bytes(int n_seqs, int n_tokens, int max_q_len, int n_heads,
                                   int n_kv_heads, int head_dim) {
-    (void)n_seqs, (void)n_tokens, (void)max_q_len, (void)n_heads, (void)n_kv_heads, (void)head_dim;
+    (void)n_seqs, (void)n_tokens;
+    const long long rows = (long long)max_q_len * (n_heads / n_kv_heads);
+    // never less than a call of fewer rows needs, so that one workspace serves both
+    if (head_dim == 64 || head_dim == 128)
+        return paged_decode_work_bytes((int)std::min<long long>(rows, kDecodeRows), head_dim);
     return 16;
 }
 
 int launch_paged_attention(const PagedAttnArgs &a, cudaStream_t st) {
     if (a.b.n_tokens == 0 || a.b.n_seqs == 0) return TQB200_OK;
+    const long long rows = (long long)a.b.max_q_len * (a.n_heads / a.n_kv_heads);
+    if (a.aligned && (a.head_dim == 64 || a.head_dim == 128) && rows <= kDecodeRows)
+        return rows > 0 ? launch_paged_decode(a, (int)rows, st) : TQB200_OK;
     if (a.type == TQB200_EL_F32)
         return a.cache_type == TQB200_EL_F32 ? launch_any<float, float>(a, st) : launch_any<float, __half>(a, st);
     if (a.type == TQB200_EL_F16) return launch_any<__half, __half>(a, st);

@@ -40,12 +40,10 @@ int check_place(const char *op, const char *name, const void *p, int dev) {
     return TQB200_OK;
 }
 int current_device(int *dev) {
-    int n = 0;
-    if (cudaGetDeviceCount(&n) != cudaSuccess || n == 0) {
+    if (cudaGetDevice(dev) != cudaSuccess) {
         cudaGetLastError();
         return set_error(TQB200_ERR_NO_DEVICE, "no CUDA device visible");
     }
-    TQ_CUDA_TRY(cudaGetDevice(dev));
     return TQB200_OK;
 }
 

@@ -1,0 +1,707 @@
+// paged_decode.cu — causal attention of few new rows (single tokens, or a handful of them per
+// sequence: at most 16 rows of queries per KV head) over a paged KV cache, sm_100a.
+//
+// Bound: HBM (every key and value is read once and used by the group's 1..16 query rows only),
+// or latency for short contexts.  A tcgen05 tile would spend 128 rows on these few, and its
+// operands would have to pass through shared memory; here keys and values go from global
+// memory into the registers of the warp that uses them, 16 bytes a lane, and never touch
+// shared memory.  The products run on mma.sync with the KEYS as the 16 rows and the queries as
+// the 8 columns (transposed products):
+//   S^T [16 keys x 8 rows] = K [16 x D] Q^T [D x 8],   O^T [D x 8] += V^T [D x 16] P^T [16 x 8].
+//  * A dot product does not care about the order of its terms, so lane (g, t) of the A operand
+//    (row g, columns 2t, 2t+1, 2t+8, 2t+9) takes dimensions 8(t + 4j) .. + 7 of key g: one
+//    16-byte load feeds two products, and the queries are laid out alike.
+//  * V^T as the A operand wants pairs of keys for one dimension: lane (g, t) loads dimensions
+//    8g .. 8g+7 of keys 2t, 2t+1, 2t+8, 2t+9 and interleaves the halves of two keys' words.
+//  * P^T as the B operand is the 8x8 transpose of the S^T accumulator (movmatrix).
+//  * fp32 activations over an fp16 cache: q is scaled per row by a power of two (its largest
+//    value to 2^13..2^14) and split into two fp16 (hi + lo: 22 bits), the weights likewise.
+//  * fp32 cache: tf32 products of operands split in two (hi hi + hi lo + lo hi: 2^-21 of the
+//    product), the accumulators transposed by shuffles.
+// Softmax: each warp keeps its own running maximum per row (shared by the warp's lanes),
+// raised only when a score passes it by 2^4 (one vote per 16 keys; else no shuffles), so
+// weights are at most 2^4; they carry a factor 2^6 that keeps small ones out of fp16's
+// subnormals.  Sums and accumulators are fp32.  The next 16 keys (and then values) are in
+// flight while the present ones are used; page numbers are read one step further ahead.
+#include <algorithm>
+#include <type_traits>
+
+#include "paged.cuh"
+
+namespace tqb200 {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kSub = 16;                // keys of a warp's step
+constexpr int kTile = kSub * kWarps;    // keys of a CTA's step: the unit of the split
+constexpr float kRaise = 4.0f;          // log2 by which a score may pass the running maximum
+constexpr float kLift = 6.0f;           // log2 of the weights' common factor
+
+struct DecodeParams {
+    PagedAttnArgs A;
+    unsigned *tickets;
+    float *parts;     // [2 grid][rows][HD + 2]: accumulators, then maximum, sum
+    int min_quota;
+};
+
+// ---------------------------------------------------------------- mma.sync
+template <typename C>
+__device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                      uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same<C, __half>::value)
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+// tf32 keeps 10 bits after the point: hi is x cut there (exact), lo what is left, cut likewise
+__device__ __forceinline__ void tf32_split(float x, uint32_t &hi, uint32_t &lo) {
+    hi = __float_as_uint(x) & 0xffffe000u;
+    lo = __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u;
+}
+template <typename C>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (std::is_same<C, __half>::value) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+}
+// hi = the fp16 of (a, b), lo = the fp16 of what is left
+__device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t &lo) {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+    hi = *reinterpret_cast<const uint32_t *>(&h);
+    lo = *reinterpret_cast<const uint32_t *>(&l);
+}
+__device__ __forceinline__ uint4 ld16(const char *p) {  // read once
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint32_t word(const uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+
+// Any infinity or NaN among the elements of four words.
+template <typename C>
+__device__ __forceinline__ bool non_finite(const uint4 &v) {
+    constexpr uint32_t e = std::is_same<C, float>::value ? 0x7f800000u : std::is_same<C, __half>::value ? 0x7c00u : 0x7f80u;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t w = word(v, i);
+        if constexpr (std::is_same<C, float>::value) bad |= (w & e) == e;
+        else bad |= (w & e) == e || ((w >> 16) & e) == e;
+    }
+    return bad;
+}
+
+// ---------------------------------------------------------------- the line of tiles
+struct Place {
+    long long total, quota, first;  // tiles in all, per CTA; the first tile of sequence `seq`
+    int seq;                        // where this CTA's range starts
+};
+
+__device__ __forceinline__ long long seq_tiles(const PagedAttnArgs &A, const SeqInfo &q) {
+    if (!q.ok || q.n == 0) return 0;
+    return (long long)A.n_kv_heads * ((max(q.len, 1) + kTile - 1) / kTile);
+}
+
+__device__ Place find_place(const DecodeParams &P) {
+    __shared__ long long s_sum[kWarps];
+    __shared__ long long s_first;
+    __shared__ int s_seq;
+    const PagedAttnArgs &A = P.A;
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const int per = (A.b.n_seqs + kThreads - 1) / kThreads;
+    const int s0 = min(A.b.n_seqs, t * per), s1 = min(A.b.n_seqs, s0 + per);
+    long long mine = 0;
+    for (int s = s0; s < s1; ++s) {
+        const SeqInfo q = seq_info(A.b, s);
+        if (!q.ok && blockIdx.x == 0) report(A.status, TQB200_PAGED_BAD_SEQ);
+        mine += seq_tiles(A, q);
+    }
+    long long inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long u = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += u;
+    }
+    if (lane == 31) s_sum[warp] = inc;
+    if (t == 0) s_seq = A.b.n_seqs;
+    __syncthreads();
+    Place p;
+    long long before = inc - mine;
+    p.total = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) before += s_sum[w];
+        p.total += s_sum[w];
+    }
+    p.quota = max((p.total + gridDim.x - 1) / gridDim.x, (long long)P.min_quota);
+    const long long at = blockIdx.x * p.quota;
+    if (at >= before && at < before + mine) {  // one thread, where the range is not empty
+        for (int s = s0; s < s1; ++s) {
+            const long long n = seq_tiles(A, seq_info(A.b, s));
+            if (at < before + n) {
+                s_seq = s;
+                s_first = before;
+                break;
+            }
+            before += n;
+        }
+    }
+    __syncthreads();
+    p.seq = s_seq;
+    p.first = s_first;
+    return p;
+}
+
+// ---------------------------------------------------------------- the kernel
+// T activations, C cache, D head_dim, NB blocks of 8 query rows.
+template <typename T, typename C, int D, int NB>
+__global__ void __launch_bounds__(kThreads) paged_decode_kernel(const __grid_constant__ DecodeParams P) {
+    constexpr bool F32 = std::is_same<C, float>::value;
+    constexpr bool SPLIT = !F32 && std::is_same<T, float>::value;  // hi + lo fp16 operands
+    constexpr int QS = F32 || SPLIT ? 2 : 1;
+    constexpr int ROWS = 8 * NB;
+    constexpr int EL = 16 / sizeof(C);     // elements of a 16-byte load
+    constexpr int KC = D / (4 * EL);       // loads per key
+    constexpr int VC = D / (8 * EL);       // loads per value row
+    constexpr int MT = D / 16;             // 16-dimension tiles of O^T
+    constexpr bool QREG = NB * QS * KC <= 4;  // query operands kept in registers
+    const PagedAttnArgs &A = P.A;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
+
+    // one buffer, in turn: the query operands while the item's tiles are read, the warps'
+    // accumulators at its end, the weights of up to 128 parts when they are joined
+    constexpr size_t kBuf = std::max({sizeof(float) * kWarps * ROWS * D, sizeof(uint4) * QS * NB * KC * 32,
+                                      sizeof(float) * ROWS * kThreads});
+    __shared__ __align__(16) char s_buf[kBuf];
+    auto &s_o = *reinterpret_cast<float(*)[kWarps][ROWS][D]>(s_buf);
+    auto &s_q = *reinterpret_cast<uint4(*)[QS * NB * KC][32]>(s_buf);
+    auto &s_w = *reinterpret_cast<float(*)[ROWS][kThreads]>(s_buf);
+    __shared__ float s_m[kWarps][ROWS], s_l[kWarps][ROWS];
+    __shared__ float s_c[ROWS];
+    __shared__ unsigned s_last;
+
+    const Place place = find_place(P);
+    long long at = blockIdx.x * place.quota;
+    const long long end = min(at + place.quota, place.total);
+    if (at >= end) return;  // uniform
+    int seq = place.seq;
+    long long seq_first = place.first;
+    const int G = A.n_heads / A.n_kv_heads;
+
+    while (at < end) {
+        // ---- the item at `at`: sequence, KV head, its tiles [u0, u0 + tiles) of the line
+        SeqInfo q = seq_info(A.b, seq);
+        long long n_seq = seq_tiles(A, q);
+        while (at >= seq_first + n_seq) {  // sequences without rows have no tiles
+            seq_first += n_seq;
+            ++seq;
+            q = seq_info(A.b, seq);
+            n_seq = seq_tiles(A, q);
+        }
+        const int tiles = (max(q.len, 1) + kTile - 1) / kTile;
+        const int head = (int)((at - seq_first) / tiles);
+        const long long u0 = seq_first + (long long)head * tiles;
+        const int ta = (int)(at - u0), tb = (int)min((long long)tiles, end - u0);
+        const int rows = q.n * G;
+        const int p0 = q.len - q.n;  // position of the first row
+        const int *table = A.b.table + (long long)seq * A.b.table_stride;
+        auto row_q = [&](int r) {
+            return (const T *)A.q + (long long)(q.q0 + r / G) * A.q_stride + (long long)(head * G + r % G) * D;
+        };
+
+        // ---- page offsets of a step's 16 keys: lane l (mod 16) has key l
+        auto page_of = [&](int tile) -> int {  // the page number, read ahead
+            const int x = tile * kTile + warp * kSub + (lane & 15);
+            return tile < tb && x < q.len ? __ldg(table + A.kv.page.div((uint32_t)x)) : -1;
+        };
+        int bad_page = 0;
+        auto offset_of = [&](int tile, int page) -> long long {
+            const int x = tile * kTile + warp * kSub + (lane & 15);
+            if (tile >= tb || x >= q.len) return -1;
+            if ((unsigned)page >= (unsigned)A.kv.n_pages) {
+                bad_page = 1;
+                return -1;
+            }
+            const int slot = x - (int)(A.kv.page.div((uint32_t)x) * A.kv.page.d);
+            return (page * A.kv.page_stride + head * A.kv.head_stride + slot * A.kv.slot_stride) * (long long)sizeof(C);
+        };
+        uint4 kr[2][KC], vr[4][VC];
+        // key g and g + 8 of 16
+        auto load_k = [&](long long off) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const long long o = __shfl_sync(0xffffffffu, off, g + 8 * h);
+                const char *p = A.kv.k + o + t4 * 16;
+#pragma unroll
+                for (int j = 0; j < KC; ++j) kr[h][j] = o >= 0 ? ld16(p + j * 64) : make_uint4(0, 0, 0, 0);
+            }
+        };
+        // values of keys 2t, 2t+1, 2t+8, 2t+9 (16 bits), t, t+4, t+8, t+12 (fp32)
+        auto v_key = [&](int i) { return F32 ? t4 + 4 * i : 2 * t4 + (i & 1) + 8 * (i >> 1); };
+        auto load_v = [&](long long off) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const long long o = __shfl_sync(0xffffffffu, off, v_key(i));
+                const char *p = A.kv.v + o + g * 16;
+#pragma unroll
+                for (int j = 0; j < VC; ++j) vr[i][j] = o >= 0 ? ld16(p + j * 128) : make_uint4(0, 0, 0, 0);
+            }
+        };
+        int page1 = page_of(ta);
+        long long off = offset_of(ta, page1);
+        page1 = page_of(ta + 1);
+        load_k(off);
+        load_v(off);
+
+        // ---- queries: lane (g, t) holds row 8 nb + g, dimensions EL (t + 4 j) .. of it
+        uint4 qr[QREG ? QS * NB * KC : 1];
+        float c[NB][2];   // log2(e) * scale (* 2^-row scale) of this lane's two columns per block
+        int see[NB][2];   // last position that the column's row sees, -1: none
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            const int r = 8 * nb + g;
+            float up = 1.0f, c_row = A.scale * kLog2e;
+            if (QREG || warp == (nb & (kWarps - 1))) {
+                if constexpr (std::is_same<T, float>::value) {
+                    float x[KC][EL];
+                    const float *src = r < rows ? row_q(r) + t4 * EL : nullptr;
+                    float most = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < KC; ++j)
+#pragma unroll
+                        for (int e = 0; e < EL; e += 4) {
+                            const float4 f = src ? *reinterpret_cast<const float4 *>(src + j * 4 * EL + e)
+                                                 : make_float4(0, 0, 0, 0);
+                            x[j][e] = f.x, x[j][e + 1] = f.y, x[j][e + 2] = f.z, x[j][e + 3] = f.w;
+                            most = fmaxf(most, fmaxf(fmaxf(fabsf(f.x), fabsf(f.y)), fmaxf(fabsf(f.z), fabsf(f.w))));
+                        }
+                    if constexpr (SPLIT) {
+                        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                        // most in [2^(e-127), 2^(e-126)) goes to [2^13, 2^14)
+                        const int e = max(14, min(254, (int)(__float_as_uint(most) >> 23)));
+                        up = __uint_as_float((uint32_t)(254 + 13 - e) << 23);
+                        c_row = c_row / up;
+                    }
+#pragma unroll
+                    for (int j = 0; j < KC; ++j) {
+                        uint32_t hi[4], lo[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            if constexpr (F32) tf32_split(x[j][e], hi[e], lo[e]);
+                            else split2(x[j][2 * e] * up, x[j][2 * e + 1] * up, hi[e], lo[e]);
+                        }
+                        const uint4 h4 = make_uint4(hi[0], hi[1], hi[2], hi[3]), l4 = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                        if constexpr (QREG) {
+                            qr[nb * KC + j] = h4;
+                            qr[(NB + nb) * KC + j] = l4;
+                        } else {
+                            s_q[nb * KC + j][lane] = h4;
+                            s_q[(NB + nb) * KC + j][lane] = l4;
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < KC; ++j) {
+                        const uint4 v = r < rows ? *reinterpret_cast<const uint4 *>(row_q(r) + (t4 + 4 * j) * EL)
+                                                 : make_uint4(0, 0, 0, 0);
+                        if constexpr (QREG) qr[nb * KC + j] = v;
+                        else s_q[nb * KC + j][lane] = v;
+                    }
+                }
+                if (!QREG && t4 == 0) s_c[r] = c_row;
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int col = 8 * nb + 2 * t4 + e;
+                if (QREG) c[nb][e] = __shfl_sync(0xffffffffu, c_row, (2 * t4 + e) * 4);
+                see[nb][e] = col < rows ? min(p0 + col / G, q.len - 1) : -1;
+            }
+        }
+        if (!QREG) {
+            __syncthreads();
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) c[nb][e] = s_c[8 * nb + 2 * t4 + e];
+        }
+        auto q_op = [&](int s, int nb, int j) -> uint4 {
+            if constexpr (QREG) return qr[(s * NB + nb) * KC + j];
+            else return s_q[(s * NB + nb) * KC + j][lane];
+        };
+
+        float o[NB][MT][4];
+        float m[NB][2], l[NB][2];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[nb][i][e] = 0.0f;
+            m[nb][0] = m[nb][1] = -INFINITY;
+            l[nb][0] = l[nb][1] = 0.0f;
+        }
+        bool poison = false;  // an infinity or NaN among values that some row of the item may not see
+
+        for (int tile = ta; tile < tb; ++tile) {
+            const int x0 = tile * kTile + warp * kSub;
+            const long long next = offset_of(tile + 1, page1);
+            page1 = page_of(tile + 2);
+            const unsigned have = __ballot_sync(0xffffffffu, off >= 0);
+            off = next;
+            // ---- scores: s[0], s[1] key g with columns 2t, 2t+1; s[2], s[3] key g + 8
+            float s[NB][4];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[nb][e] = 0.0f;
+#pragma unroll
+                for (int j = 0; j < KC; ++j) {
+                    if constexpr (F32) {
+                        const uint4 qh = q_op(0, nb, j), ql = q_op(1, nb, j);
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            uint32_t hi[4], lo[4];
+                            tf32_split(__uint_as_float(word(kr[0][j], 2 * u)), hi[0], lo[0]);
+                            tf32_split(__uint_as_float(word(kr[1][j], 2 * u)), hi[1], lo[1]);
+                            tf32_split(__uint_as_float(word(kr[0][j], 2 * u + 1)), hi[2], lo[2]);
+                            tf32_split(__uint_as_float(word(kr[1][j], 2 * u + 1)), hi[3], lo[3]);
+                            mma_tf32(s[nb], lo, word(qh, 2 * u), word(qh, 2 * u + 1));
+                            mma_tf32(s[nb], hi, word(ql, 2 * u), word(ql, 2 * u + 1));
+                            mma_tf32(s[nb], hi, word(qh, 2 * u), word(qh, 2 * u + 1));
+                        }
+                    } else {
+#pragma unroll
+                        for (int sp = QS - 1; sp >= 0; --sp) {
+                            const uint4 b = q_op(sp, nb, j);
+                            mma16<C>(s[nb], kr[0][j].x, kr[1][j].x, kr[0][j].y, kr[1][j].y, b.x, b.y);
+                            mma16<C>(s[nb], kr[0][j].z, kr[1][j].z, kr[0][j].w, kr[1][j].w, b.z, b.w);
+                        }
+                    }
+                }
+            }
+            load_k(off);
+            // ---- masks and the running maximum
+            bool raise = false;
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int x = x0 + g + 8 * (e >> 1);
+                    const bool ok = x <= see[nb][e & 1] && ((have >> (g + 8 * (e >> 1))) & 1u);
+                    s[nb][e] = ok ? s[nb][e] * c[nb][e & 1] : -INFINITY;
+                    raise |= s[nb][e] > m[nb][e & 1] + kRaise;
+                }
+            if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float mx = fmaxf(s[nb][e], s[nb][e + 2]);
+#pragma unroll
+                        for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+                        if (mx > m[nb][e]) {
+                            const float f = ex2(m[nb][e] - mx);  // 0 from -inf
+                            m[nb][e] = mx;
+                            l[nb][e] *= f;
+#pragma unroll
+                            for (int i = 0; i < MT; ++i) o[nb][i][e] *= f, o[nb][i][e + 2] *= f;
+                        }
+                    }
+            }
+            // ---- weights
+            uint32_t pb[QS][NB][2][2];  // B operands: [split][block][k8 step (fp32)][b0, b1]; 16 bits: [..][0]
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                float p[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float base = m[nb][e & 1] == -INFINITY ? 0.0f : m[nb][e & 1] - kLift;
+                    p[e] = ex2(s[nb][e] - base);
+                    l[nb][e & 1] += p[e];
+                }
+                if constexpr (F32) {
+#pragma unroll
+                    for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+                        for (int b = 0; b < 2; ++b) {
+                            const int src = (t4 + 4 * b) * 4 + (g >> 1);
+                            const float v0 = __shfl_sync(0xffffffffu, p[2 * kk], src);
+                            const float v1 = __shfl_sync(0xffffffffu, p[2 * kk + 1], src);
+                            tf32_split((g & 1) ? v1 : v0, pb[0][nb][kk][b], pb[1][nb][kk][b]);
+                        }
+                } else if constexpr (SPLIT) {
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        uint32_t hi, lo;
+                        split2(p[2 * b], p[2 * b + 1], hi, lo);
+                        pb[0][nb][0][b] = transpose8x8(hi);
+                        pb[1][nb][0][b] = transpose8x8(lo);
+                    }
+                } else {
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) pb[0][nb][0][b] = transpose8x8(pack2<C>(p[2 * b], p[2 * b + 1]));
+                }
+            }
+            // ---- values.  A weight of 0 does not hide an infinity or NaN: where a row of the
+            // item may not see a value, look for them, and take the item's slow pass if any
+            if (q.n > 1 && x0 + kSub - 1 > p0) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < VC; ++j) poison |= x0 + v_key(i) > p0 && non_finite<C>(vr[i][j]);
+            }
+            if constexpr (F32) {
+#pragma unroll
+                for (int j = 0; j < VC; ++j)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int kk = 0; kk < 2; ++kk) {
+                            uint32_t hi[4], lo[4];
+                            tf32_split(__uint_as_float(word(vr[2 * kk][j], 2 * i)), hi[0], lo[0]);
+                            tf32_split(__uint_as_float(word(vr[2 * kk][j], 2 * i + 1)), hi[1], lo[1]);
+                            tf32_split(__uint_as_float(word(vr[2 * kk + 1][j], 2 * i)), hi[2], lo[2]);
+                            tf32_split(__uint_as_float(word(vr[2 * kk + 1][j], 2 * i + 1)), hi[3], lo[3]);
+#pragma unroll
+                            for (int nb = 0; nb < NB; ++nb) {
+                                mma_tf32(o[nb][j * 2 + i], lo, pb[0][nb][kk][0], pb[0][nb][kk][1]);
+                                mma_tf32(o[nb][j * 2 + i], hi, pb[1][nb][kk][0], pb[1][nb][kk][1]);
+                                mma_tf32(o[nb][j * 2 + i], hi, pb[0][nb][kk][0], pb[0][nb][kk][1]);
+                            }
+                        }
+            } else {
+#pragma unroll
+                for (int j = 0; j < VC; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t wa = word(vr[0][j], i), wb = word(vr[1][j], i);
+                        const uint32_t wc = word(vr[2][j], i), wd = word(vr[3][j], i);
+                        const uint32_t a0 = __byte_perm(wa, wb, 0x5410), a1 = __byte_perm(wa, wb, 0x7632);
+                        const uint32_t a2 = __byte_perm(wc, wd, 0x5410), a3 = __byte_perm(wc, wd, 0x7632);
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                            for (int sp = QS - 1; sp >= 0; --sp)
+                                mma16<C>(o[nb][j * 4 + i], a0, a1, a2, a3, pb[sp][nb][0][0], pb[sp][nb][0][1]);
+                    }
+            }
+            load_v(off);
+        }
+        if (__any_sync(0xffffffffu, bad_page) && lane == 0) report(A.status, TQB200_PAGED_BAD_PAGE);
+
+        // ---- the warps' parts, joined through shared memory
+        const bool slow = __syncthreads_or(poison);  // also: the previous item's reads of s_o are done
+        if (slow) {
+            for (int r = warp; r < ROWS; r += kWarps) {
+                float mr = -INFINITY, lr = 0.0f, orow[8];
+                if (r < rows) {
+                    const int x1 = min(min(tb * kTile, q.len), p0 + r / G + 1);
+                    row_pass<T, C>(A, row_q(r), seq, head, ta * kTile, x1, mr, lr, orow);
+                    const float lift = exp2f(kLift);
+                    lr *= lift;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) orow[j] *= lift;
+                }
+                for (int w = 0; w < kWarps; ++w) {
+                    if (lane == 0) s_m[w][r] = w ? -INFINITY : mr, s_l[w][r] = w ? 0.0f : lr;
+#pragma unroll
+                    for (int j = 0; j < D / 32; ++j) s_o[w][r][lane + 32 * j] = w || r >= rows ? 0.0f : orow[j];
+                }
+            }
+        } else {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) l[nb][e] += __shfl_xor_sync(0xffffffffu, l[nb][e], d);
+                    if (g == 0) {
+                        s_m[warp][8 * nb + 2 * t4 + e] = m[nb][e];
+                        s_l[warp][8 * nb + 2 * t4 + e] = l[nb][e];
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    constexpr int TJ = F32 ? 2 : 4;  // tiles per load
+                    const int d = (i / TJ) * 8 * EL + EL * g + 2 * (i % TJ);
+                    *reinterpret_cast<float2 *>(&s_o[warp][8 * nb + 2 * t4][d]) = make_float2(o[nb][i][0], o[nb][i][2]);
+                    *reinterpret_cast<float2 *>(&s_o[warp][8 * nb + 2 * t4 + 1][d]) = make_float2(o[nb][i][1], o[nb][i][3]);
+                }
+            }
+        }
+        __syncthreads();
+        const bool whole = ta == 0 && tb == tiles;
+        // slot of this CTA's part: the item continues from an earlier CTA (or starts the range)
+        float *part = P.parts + (2 * (long long)blockIdx.x + (at == blockIdx.x * place.quota ? 0 : 1)) * ROWS * (D + 2);
+        for (int i = tid; i < rows * (D / 4); i += kThreads) {
+            const int r = i / (D / 4), d = (i % (D / 4)) * 4;
+            float M = s_m[0][r];
+#pragma unroll
+            for (int w = 1; w < kWarps; ++w) M = fmaxf(M, s_m[w][r]);
+            const float base = M == -INFINITY ? 0.0f : M;
+            float L = 0.0f;
+            float4 v = make_float4(0, 0, 0, 0);
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float f = ex2(s_m[w][r] - base);
+                const float4 x = *reinterpret_cast<const float4 *>(&s_o[w][r][d]);
+                L = fmaf(f, s_l[w][r], L);
+                v.x = fmaf(f, x.x, v.x), v.y = fmaf(f, x.y, v.y), v.z = fmaf(f, x.z, v.z), v.w = fmaf(f, x.w, v.w);
+            }
+            if (whole) {
+                const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+                const float y[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
+                ElVec<T, 4> ov;
+                ov.set(y);
+                ov.store((T *)A.out + (long long)(q.q0 + r / G) * A.out_stride + (long long)(head * G + r % G) * D + d);
+            } else {
+                *reinterpret_cast<float4 *>(part + r * D + d) = v;
+                if (d == 0) part[ROWS * D + r] = M, part[ROWS * D + ROWS + r] = L;
+            }
+        }
+        if (!whole) {
+            // ---- the item's parts from CTAs c0 .. c1; the last to arrive joins them in order
+            const long long quota = place.quota;
+            const int c0 = (int)(u0 / quota), c1 = (int)((u0 + tiles - 1) / quota);
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) s_last = atomicAdd(&P.tickets[c0], 1u) == (unsigned)(c1 - c0);
+            __syncthreads();
+            if (s_last) {  // uniform
+                __threadfence();
+                auto part_of = [&](int cta) {
+                    return P.parts + (2 * (long long)cta + ((long long)cta * quota >= u0 ? 0 : 1)) * ROWS * (D + 2);
+                };
+                // every row's maximum over the parts (s_m[0]) and sum (s_l[0])
+                for (int r = warp; r < rows; r += kWarps) {
+                    float M = -INFINITY;
+                    for (int i = c0 + lane; i <= c1; i += 32) M = fmaxf(M, __ldcg(part_of(i) + ROWS * D + r));
+#pragma unroll
+                    for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+                    const float base = M == -INFINITY ? 0.0f : M;
+                    float L = 0.0f;
+                    for (int i = c0 + lane; i <= c1; i += 32) {
+                        const float *pp = part_of(i) + ROWS * D;
+                        L = fmaf(ex2(__ldcg(pp + r) - base), __ldcg(pp + ROWS + r), L);
+                    }
+                    L = warp_sum(L);
+                    if (lane == 0) s_m[0][r] = base, s_l[0][r] = L;
+                }
+                __syncthreads();
+                constexpr int PER = ROWS * D / 4 / kThreads;  // float4 of the result per thread
+                float4 acc[PER];
+#pragma unroll
+                for (int k = 0; k < PER; ++k) acc[k] = make_float4(0, 0, 0, 0);
+                for (int b = c0; b <= c1; b += kThreads) {
+                    const int cnt = min(kThreads, c1 + 1 - b);
+                    for (int i = tid; i < cnt * rows; i += kThreads) {
+                        const int r = i / cnt, w = i % cnt;
+                        s_w[r][w] = ex2(__ldcg(part_of(b + w) + ROWS * D + r) - s_m[0][r]);
+                    }
+                    __syncthreads();
+#pragma unroll
+                    for (int k = 0; k < PER; ++k) {
+                        const int i = tid + k * kThreads, r = i / (D / 4), d = (i % (D / 4)) * 4;
+                        if (r < rows) {
+#pragma unroll 8
+                            for (int w = 0; w < cnt; ++w) {
+                                const float4 x = __ldcg(reinterpret_cast<const float4 *>(part_of(b + w) + r * D + d));
+                                const float f = s_w[r][w];
+                                acc[k].x = fmaf(f, x.x, acc[k].x), acc[k].y = fmaf(f, x.y, acc[k].y);
+                                acc[k].z = fmaf(f, x.z, acc[k].z), acc[k].w = fmaf(f, x.w, acc[k].w);
+                            }
+                        }
+                    }
+                    __syncthreads();
+                }
+#pragma unroll
+                for (int k = 0; k < PER; ++k) {
+                    const int i = tid + k * kThreads, r = i / (D / 4), d = (i % (D / 4)) * 4;
+                    if (r < rows) {
+                        const float L = s_l[0][r], inv = L == 0.0f ? 0.0f : 1.0f / L;
+                        const float y[4] = {acc[k].x * inv, acc[k].y * inv, acc[k].z * inv, acc[k].w * inv};
+                        ElVec<T, 4> ov;
+                        ov.set(y);
+                        ov.store((T *)A.out + (long long)(q.q0 + r / G) * A.out_stride + (long long)(head * G + r % G) * D + d);
+                    }
+                }
+                if (tid == 0) P.tickets[c0] = 0;  // ready for the next call
+            }
+        }
+        at = u0 + tb;
+        __syncthreads();  // shared memory free for the next item
+    }
+}
+
+template <typename T, typename C, int D, int NB>
+int launch_decode_t(const PagedAttnArgs &a, cudaStream_t st) {
+    static std::atomic<int> s_occ{0};
+    int occ = s_occ.load();
+    auto k = paged_decode_kernel<T, C, D, NB>;
+    if (!occ) {
+        TQ_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, k, kThreads, 0));
+        TQ_CHECK_ARG(occ >= 1, "paged_attention: the decode kernel does not fit an SM");
+        s_occ.store(occ);
+    }
+    DecodeParams P{};
+    P.A = a;
+    P.tickets = (unsigned *)a.work;
+    P.parts = (float *)((char *)a.work + kSplitTicketBytes);
+    P.min_quota = 2;
+    // no more CTAs than there can be tiles
+    const long long most = (long long)a.b.n_seqs * a.n_kv_heads * ((std::max(1, a.b.max_len) + kTile - 1) / kTile);
+    const int grid = (int)std::min<long long>({(long long)num_sms() * std::min(occ, 4), most, kSplitMaxCtas});
+    k<<<grid, kThreads, 0, st>>>(P);
+    TQ_CUDA_TRY(cudaGetLastError());
+    return TQB200_OK;
+}
+
+template <typename T, typename C>
+int launch_decode_c(const PagedAttnArgs &a, int rows, cudaStream_t st) {
+    if (a.head_dim == 64)
+        return rows <= 8 ? launch_decode_t<T, C, 64, 1>(a, st) : launch_decode_t<T, C, 64, 2>(a, st);
+    return rows <= 8 ? launch_decode_t<T, C, 128, 1>(a, st) : launch_decode_t<T, C, 128, 2>(a, st);
+}
+
+}  // namespace
+
+size_t paged_decode_work_bytes(int rows, int head_dim) {
+    const size_t ctas = std::min(4 * num_sms(), kSplitMaxCtas);
+    return kSplitTicketBytes + 2 * ctas * (rows <= 8 ? 8 : 16) * (size_t)(head_dim + 2) * 4;
+}
+
+int launch_paged_decode(const PagedAttnArgs &a, int rows, cudaStream_t st) {
+    if (a.type == TQB200_EL_F32)
+        return a.cache_type == TQB200_EL_F32 ? launch_decode_c<float, float>(a, rows, st)
+                                             : launch_decode_c<float, __half>(a, rows, st);
+    if (a.type == TQB200_EL_F16) return launch_decode_c<__half, __half>(a, rows, st);
+    return launch_decode_c<__nv_bfloat16, __nv_bfloat16>(a, rows, st);
+}
+
+}  // namespace tqb200
