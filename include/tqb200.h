@@ -307,10 +307,10 @@ int tqb200_dev_paged_append(const void *q, const void *k, const void *v, void *q
  * with p the row's position.  A row that sees no position (p < 0, or all its pages bad) gets
  * zeros.  out may not overlap q.  The workspace holds
  * tqb200_paged_attention_workspace_bytes() bytes, 16-byte aligned, zero before its first
- * call; every call leaves it ready for the next.  The bytes depend on n_heads, n_kv_heads,
- * head_dim and max_q_len and do not grow when max_q_len shrinks, so a workspace for the largest
- * chunk also serves single tokens.  One workspace serves any calls that do not overlap on the
- * GPU (captured graphs included); calls that may overlap need one each. */
+ * call; every call leaves it ready for the next.  The bytes depend on the
+ * device and head_dim alone, so one workspace serves chunks and single tokens, and any calls
+ * that do not overlap on the GPU (captured graphs included); calls that may overlap need one
+ * each. */
 size_t tqb200_paged_attention_workspace_bytes(const tqb200_paged_cache *cache,
                                               const tqb200_paged_batch *batch, int n_heads);
 int tqb200_dev_paged_attention(const void *q, void *out, int type, int n_heads, long long q_stride,

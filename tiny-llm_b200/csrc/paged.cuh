@@ -240,25 +240,213 @@ __device__ __noinline__ void row_pass(const PagedAttnArgs &A, const T *q, int se
 }
 
 // ---------------------------------------------------------------- split attention
-// The work of a call is one line of tiles: for every sequence with rows, for every KV head,
-// (for every block of query rows,) the tiles of positions it reads.  CTA c takes tiles
-// [c quota, (c+1) quota), so every CTA reads equally many whatever the lengths are; the parts
-// of a (sequence, head, rows) item that lies in several CTAs are joined by the last of them
-// to arrive, in the order of the line (the result does not depend on who is last).  The item's
-// first CTA names its ticket; a CTA leaves at most two parts: that of the item it begins in
-// the middle of (slot 2c) and that of the item it ends in the middle of (slot 2c + 1).
+// The work of a call is one line of tiles.  An item is a block of `tq` tokens of one sequence
+// with the query heads of one KV head (or some of them: `heads` such sets per sequence); it
+// reads KT positions per tile, up to its last token's own.  The line has the sequences in
+// order, in each the head sets, in each the token blocks.  CTA c takes tiles
+// [c quota, (c+1) quota), so every CTA reads equally many whatever the lengths are; an item
+// that lies in several CTAs is joined by the last of them to arrive, in the order of the line
+// (the result does not depend on who is last).  Such an item's first CTA names its ticket; a
+// CTA leaves at most two parts: of the item that it begins in the middle of (slot 2c) and of
+// the one that it ends in the middle of (slot 2c + 1).  Where the quota is below `whole_below`
+// tiles, joining would cost more than it saves: CTA c then takes the whole of every item that
+// begins in its range.
 constexpr int kSplitMaxCtas = 1024;
 constexpr size_t kSplitTicketBytes = kSplitMaxCtas * 4;  // head of the workspace, zero between calls
+
+struct LineShape {
+    int tq, heads;
+    int min_quota, whole_below;
+};
+
+// Sum of floor((a i + b) / m) over 0 <= i < n: lattice points under a line, by exchanging the
+// axes as in Euclid's algorithm (Graham, Knuth, Patashnik, Concrete Mathematics, 3.5).  With
+// a, b < m the line reaches height h = floor((a (n-1) + b) / m); the points (i, y), 1 <= y <= h,
+// under it are, per y, those with i >= (m y - b) / a:  n h - sum_y ceil((m y - b) / a), and
+// ceil((m y - b) / a) = floor((m (y - 1) + m - b + a - 1) / a).
+__device__ inline long long floor_line_sum(long long n, long long a, long long b, long long m) {
+    long long sum = 0, sign = 1;
+    while (n > 0) {
+        if (a >= m || b >= m) {
+            sum += sign * ((a / m) * (n * (n - 1) / 2) + (b / m) * n);
+            a %= m;
+            b %= m;
+        }
+        const long long h = (a * (n - 1) + b) / m;
+        if (h == 0) break;
+        sum += sign * n * h;
+        sign = -sign;
+        const long long b2 = m - b + a - 1;
+        n = h;
+        b = b2;
+        const long long m2 = a;
+        a = m;
+        m = m2;
+    }
+    return sum;
+}
+
+template <int KT>
+struct Line {
+    // tiles of token block b of `nb`: positions up to its last token's, at least one tile
+    __device__ static __forceinline__ int block_tiles(const SeqInfo &q, int tq, int nb, int b) {
+        const int last = q.len - q.n + (b == nb - 1 ? q.n : (b + 1) * tq) - 1;
+        return last < 0 ? 1 : last / KT + 1;
+    }
+    __device__ static __forceinline__ int blocks(const SeqInfo &q, int tq) { return (q.n + tq - 1) / tq; }
+    // tiles of one head set
+    __device__ static __forceinline__ long long head_tiles(const SeqInfo &q, int tq) {
+        if (!q.ok || q.n == 0) return 0;
+        const int nb = blocks(q, tq);
+        long long sum = block_tiles(q, tq, nb, nb - 1);
+        if (nb > 1) {
+            const int p0 = q.len - q.n;
+            // the blocks before it: those that end before position 0 have one tile each
+            const int none = p0 < 0 ? min(nb - 1, (int)(-(long long)p0 / tq)) : 0;
+            sum += nb - 1 + floor_line_sum(nb - 1 - none, tq, (long long)p0 + (long long)none * tq + tq - 1, KT);
+        }
+        return sum;
+    }
+
+    // ---- one warp's way along its CTA's part of the line (every warp walks it for itself)
+    LineShape sh;
+    SeqInfo q;
+    long long quota, at, end, u0;  // tiles: per CTA; the next, the end of the range; the item's first
+    int seq, head, b, nb, tiles, ta, tb;
+    bool whole;                     // the items are taken whole
+
+    __device__ __forceinline__ void enter_seq(const BatchView &B, int s) {
+        seq = s;
+        q = seq_info(B, s);
+        while (!q.ok || q.n == 0) {
+            if (++seq >= B.n_seqs) return;
+            q = seq_info(B, seq);
+        }
+        head = 0;
+        b = 0;
+        nb = blocks(q, sh.tq);
+        tiles = block_tiles(q, sh.tq, nb, 0);
+    }
+    // The item after this one; seq == n_seqs behind the last.
+    __device__ __forceinline__ void step(const BatchView &B) {
+        u0 += tiles;
+        if (++b == nb) {
+            b = 0;
+            if (++head == sh.heads) {
+                if (++seq < B.n_seqs) enter_seq(B, seq);
+                return;
+            }
+        }
+        tiles = block_tiles(q, sh.tq, nb, b);
+    }
+    // The present item's part [ta, tb) for this CTA; false: the range is done.
+    __device__ __forceinline__ bool part(const BatchView &B) {
+        if (at >= end || seq >= B.n_seqs) return false;
+        ta = whole ? 0 : (int)(at - u0);
+        tb = whole ? tiles : (int)min((long long)tiles, end - u0);
+        return true;
+    }
+    __device__ __forceinline__ void next(const BatchView &B) {
+        at = u0 + tiles;
+        step(B);
+    }
+    // The CTAs that share the item: the first and the last.
+    __device__ __forceinline__ int first_cta() const { return (int)(u0 / quota); }
+    __device__ __forceinline__ int last_cta() const { return (int)((u0 + tiles - 1) / quota); }
+    __device__ __forceinline__ bool all_mine() const { return ta == 0 && tb == tiles; }
+    __device__ __forceinline__ long long slot_of(int cta) const {
+        return 2 * (long long)cta + ((long long)cta * quota >= u0 ? 0 : 1);
+    }
+
+    // Whole CTA (THREADS of it), once: the line's length, the range, the first item.
+    template <int THREADS>
+    __device__ void begin(const BatchView &B, const LineShape &shape, int *status) {
+        constexpr int WARPS = THREADS / 32;
+        __shared__ long long s_sum[WARPS], s_first;
+        __shared__ int s_seq;
+        sh = shape;
+        const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+        const int per = (B.n_seqs + THREADS - 1) / THREADS;
+        const int s0 = min(B.n_seqs, t * per), s1 = min(B.n_seqs, s0 + per);
+        long long mine = 0;
+        for (int s = s0; s < s1; ++s) {
+            const SeqInfo i = seq_info(B, s);
+            if (!i.ok && blockIdx.x == 0) report(status, TQB200_PAGED_BAD_SEQ);
+            mine += sh.heads * head_tiles(i, sh.tq);
+        }
+        long long inc = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long u = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += u;
+        }
+        if (lane == 31) s_sum[warp] = inc;
+        if (t == 0) s_seq = B.n_seqs;
+        __syncthreads();
+        long long before = inc - mine, total = 0;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            if (w < warp) before += s_sum[w];
+            total += s_sum[w];
+        }
+        quota = max((total + gridDim.x - 1) / gridDim.x, (long long)sh.min_quota);
+        whole = quota < sh.whole_below;
+        at = blockIdx.x * quota;
+        end = min(at + quota, total);
+        if (at < end && at >= before && at < before + mine) {  // one thread
+            for (int s = s0; s < s1; ++s) {
+                const long long n = sh.heads * head_tiles(seq_info(B, s), sh.tq);
+                if (at < before + n) {
+                    s_seq = s;
+                    s_first = before;
+                    break;
+                }
+                before += n;
+            }
+        }
+        __syncthreads();
+        seq = s_seq;
+        if (at >= end || seq >= B.n_seqs) {
+            at = end;  // nothing for this CTA
+            return;
+        }
+        // the item at `at`: head set by division, token block by a scan of 32 blocks at a time
+        enter_seq(B, seq);
+        const long long ht = head_tiles(q, sh.tq);
+        head = (int)((at - s_first) / ht);
+        u0 = s_first + head * ht;
+        long long off = at - u0;
+        for (int b0 = 0; b0 < nb; b0 += 32) {
+            const int n = b0 + lane < nb ? block_tiles(q, sh.tq, nb, b0 + lane) : 0;
+            int sum = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += u;
+            }
+            const unsigned past = __ballot_sync(0xffffffffu, off < sum);
+            if (past) {
+                const int l = __ffs((int)past) - 1;
+                b = b0 + l;
+                tiles = __shfl_sync(0xffffffffu, n, l);
+                u0 += __shfl_sync(0xffffffffu, sum, l) - tiles;
+                break;
+            }
+            off -= __shfl_sync(0xffffffffu, sum, 31);
+            u0 += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        if (whole && at > u0) next(B);  // begun in the range before
+    }
+};
 
 int launch_qk_norm_rope(const RopeArgs &a, cudaStream_t st);
 int launch_paged_append(const RopeArgs &a, const PagedView &kv, int cache_type, const BatchView &b,
                         int *status, cudaStream_t st);
 int launch_paged_attention(const PagedAttnArgs &a, cudaStream_t st);
-// At most 16 query rows per KV head, head_dim 64 or 128, 16-byte aligned rows.
-int launch_paged_decode(const PagedAttnArgs &a, int rows, cudaStream_t st);
-size_t paged_decode_work_bytes(int rows, int head_dim);
+// head_dim 64 or 128, 16-byte aligned rows; blocks of up to 16 query rows.
+int launch_paged_decode(const PagedAttnArgs &a, cudaStream_t st);
+size_t paged_decode_work_bytes(int head_dim);
 constexpr int kDecodeRows = 16;
-size_t paged_attention_work_bytes(int n_seqs, int n_tokens, int max_q_len, int n_heads,
-                                  int n_kv_heads, int head_dim);
+size_t paged_attention_work_bytes(int n_heads, int n_kv_heads, int head_dim);
 
 }  // namespace tqb200

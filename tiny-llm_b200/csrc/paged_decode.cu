@@ -42,7 +42,8 @@ struct DecodeParams {
     PagedAttnArgs A;
     unsigned *tickets;
     float *parts;     // [2 grid][rows][HD + 2]: accumulators, then maximum, sum
-    int min_quota;
+    LineShape line;
+    int sets, g_set;  // sets of at most g_set query heads that a KV head's queries fall into
 };
 
 // ---------------------------------------------------------------- mma.sync
@@ -102,81 +103,6 @@ __device__ __forceinline__ uint4 ld16(const char *p) {  // read once
 }
 __device__ __forceinline__ uint32_t word(const uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
-// Any infinity or NaN among the elements of four words.
-template <typename C>
-__device__ __forceinline__ bool non_finite(const uint4 &v) {
-    constexpr uint32_t e = std::is_same<C, float>::value ? 0x7f800000u : std::is_same<C, __half>::value ? 0x7c00u : 0x7f80u;
-    bool bad = false;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t w = word(v, i);
-        if constexpr (std::is_same<C, float>::value) bad |= (w & e) == e;
-        else bad |= (w & e) == e || ((w >> 16) & e) == e;
-    }
-    return bad;
-}
-
-// ---------------------------------------------------------------- the line of tiles
-struct Place {
-    long long total, quota, first;  // tiles in all, per CTA; the first tile of sequence `seq`
-    int seq;                        // where this CTA's range starts
-};
-
-__device__ __forceinline__ long long seq_tiles(const PagedAttnArgs &A, const SeqInfo &q) {
-    if (!q.ok || q.n == 0) return 0;
-    return (long long)A.n_kv_heads * ((max(q.len, 1) + kTile - 1) / kTile);
-}
-
-__device__ Place find_place(const DecodeParams &P) {
-    __shared__ long long s_sum[kWarps];
-    __shared__ long long s_first;
-    __shared__ int s_seq;
-    const PagedAttnArgs &A = P.A;
-    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    const int per = (A.b.n_seqs + kThreads - 1) / kThreads;
-    const int s0 = min(A.b.n_seqs, t * per), s1 = min(A.b.n_seqs, s0 + per);
-    long long mine = 0;
-    for (int s = s0; s < s1; ++s) {
-        const SeqInfo q = seq_info(A.b, s);
-        if (!q.ok && blockIdx.x == 0) report(A.status, TQB200_PAGED_BAD_SEQ);
-        mine += seq_tiles(A, q);
-    }
-    long long inc = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long u = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += u;
-    }
-    if (lane == 31) s_sum[warp] = inc;
-    if (t == 0) s_seq = A.b.n_seqs;
-    __syncthreads();
-    Place p;
-    long long before = inc - mine;
-    p.total = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) before += s_sum[w];
-        p.total += s_sum[w];
-    }
-    p.quota = max((p.total + gridDim.x - 1) / gridDim.x, (long long)P.min_quota);
-    const long long at = blockIdx.x * p.quota;
-    if (at >= before && at < before + mine) {  // one thread, where the range is not empty
-        for (int s = s0; s < s1; ++s) {
-            const long long n = seq_tiles(A, seq_info(A.b, s));
-            if (at < before + n) {
-                s_seq = s;
-                s_first = before;
-                break;
-            }
-            before += n;
-        }
-    }
-    __syncthreads();
-    p.seq = s_seq;
-    p.first = s_first;
-    return p;
-}
-
 // ---------------------------------------------------------------- the kernel
 // T activations, C cache, D head_dim, NB blocks of 8 query rows.
 template <typename T, typename C, int D, int NB>
@@ -205,33 +131,24 @@ __global__ void __launch_bounds__(kThreads) paged_decode_kernel(const __grid_con
     __shared__ float s_c[ROWS];
     __shared__ unsigned s_last;
 
-    const Place place = find_place(P);
-    long long at = blockIdx.x * place.quota;
-    const long long end = min(at + place.quota, place.total);
-    if (at >= end) return;  // uniform
-    int seq = place.seq;
-    long long seq_first = place.first;
+    Line<kTile> it;
+    it.begin<kThreads>(A.b, P.line, A.status);
     const int G = A.n_heads / A.n_kv_heads;
 
-    while (at < end) {
-        // ---- the item at `at`: sequence, KV head, its tiles [u0, u0 + tiles) of the line
-        SeqInfo q = seq_info(A.b, seq);
-        long long n_seq = seq_tiles(A, q);
-        while (at >= seq_first + n_seq) {  // sequences without rows have no tiles
-            seq_first += n_seq;
-            ++seq;
-            q = seq_info(A.b, seq);
-            n_seq = seq_tiles(A, q);
-        }
-        const int tiles = (max(q.len, 1) + kTile - 1) / kTile;
-        const int head = (int)((at - seq_first) / tiles);
-        const long long u0 = seq_first + (long long)head * tiles;
-        const int ta = (int)(at - u0), tb = (int)min((long long)tiles, end - u0);
-        const int rows = q.n * G;
-        const int p0 = q.len - q.n;  // position of the first row
-        const int *table = A.b.table + (long long)seq * A.b.table_stride;
+    for (; it.part(A.b); it.next(A.b)) {
+        // ---- the item: rows (token, query head) of one KV head, tokens tok0 ..
+        const SeqInfo &q = it.q;
+        const int head = it.head / P.sets, h0 = (it.head - head * P.sets) * P.g_set;
+        const int gs = min(P.g_set, G - h0);  // query heads of this set
+        const int ta = it.ta, tb = it.tb, tok0 = it.b * P.line.tq;
+        const int rows = min(P.line.tq, q.n - tok0) * gs;
+        const int p0 = q.len - q.n + tok0;  // position of the first row
+        const int *table = A.b.table + (long long)it.seq * A.b.table_stride;
+        auto row_at = [&](int r, long long stride) {
+            return (long long)(q.q0 + tok0 + r / gs) * stride + (long long)(head * G + h0 + r % gs) * D;
+        };
         auto row_q = [&](int r) {
-            return (const T *)A.q + (long long)(q.q0 + r / G) * A.q_stride + (long long)(head * G + r % G) * D;
+            return (const T *)A.q + row_at(r, A.q_stride);
         };
 
         // ---- page offsets of a step's 16 keys: lane l (mod 16) has key l
@@ -340,7 +257,7 @@ __global__ void __launch_bounds__(kThreads) paged_decode_kernel(const __grid_con
             for (int e = 0; e < 2; ++e) {
                 const int col = 8 * nb + 2 * t4 + e;
                 if (QREG) c[nb][e] = __shfl_sync(0xffffffffu, c_row, (2 * t4 + e) * 4);
-                see[nb][e] = col < rows ? min(p0 + col / G, q.len - 1) : -1;
+                see[nb][e] = col < rows ? p0 + col / gs : -1;
             }
         }
         if (!QREG) {
@@ -366,7 +283,6 @@ __global__ void __launch_bounds__(kThreads) paged_decode_kernel(const __grid_con
             m[nb][0] = m[nb][1] = -INFINITY;
             l[nb][0] = l[nb][1] = 0.0f;
         }
-        bool poison = false;  // an infinity or NaN among values that some row of the item may not see
 
         for (int tile = ta; tile < tb; ++tile) {
             const int x0 = tile * kTile + warp * kSub;
@@ -468,14 +384,7 @@ __global__ void __launch_bounds__(kThreads) paged_decode_kernel(const __grid_con
                     for (int b = 0; b < 2; ++b) pb[0][nb][0][b] = transpose8x8(pack2<C>(p[2 * b], p[2 * b + 1]));
                 }
             }
-            // ---- values.  A weight of 0 does not hide an infinity or NaN: where a row of the
-            // item may not see a value, look for them, and take the item's slow pass if any
-            if (q.n > 1 && x0 + kSub - 1 > p0) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < VC; ++j) poison |= x0 + v_key(i) > p0 && non_finite<C>(vr[i][j]);
-            }
+            // ---- values
             if constexpr (F32) {
 #pragma unroll
                 for (int j = 0; j < VC; ++j)
@@ -516,13 +425,24 @@ __global__ void __launch_bounds__(kThreads) paged_decode_kernel(const __grid_con
         if (__any_sync(0xffffffffu, bad_page) && lane == 0) report(A.status, TQB200_PAGED_BAD_PAGE);
 
         // ---- the warps' parts, joined through shared memory
-        const bool slow = __syncthreads_or(poison);  // also: the previous item's reads of s_o are done
+        // A weight of 0 does not hide an infinity or NaN.  Where some row of the item does not see
+        // some value, results that are not finite are computed again by a pass over what the row sees.
+        bool odd = false;
+        if (q.n > 1) {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) odd |= (__float_as_uint(o[nb][i][e]) & 0x7f800000u) == 0x7f800000u;
+        }
+        const bool slow = __syncthreads_or(odd);  // also: every warp is done with the query operands
         if (slow) {
             for (int r = warp; r < ROWS; r += kWarps) {
                 float mr = -INFINITY, lr = 0.0f, orow[8];
                 if (r < rows) {
-                    const int x1 = min(min(tb * kTile, q.len), p0 + r / G + 1);
-                    row_pass<T, C>(A, row_q(r), seq, head, ta * kTile, x1, mr, lr, orow);
+                    const int x1 = min(tb * kTile, p0 + r / gs + 1);
+                    row_pass<T, C>(A, row_q(r), it.seq, head, ta * kTile, x1, mr, lr, orow);
                     const float lift = exp2f(kLift);
                     lr *= lift;
 #pragma unroll
@@ -556,9 +476,8 @@ __global__ void __launch_bounds__(kThreads) paged_decode_kernel(const __grid_con
             }
         }
         __syncthreads();
-        const bool whole = ta == 0 && tb == tiles;
-        // slot of this CTA's part: the item continues from an earlier CTA (or starts the range)
-        float *part = P.parts + (2 * (long long)blockIdx.x + (at == blockIdx.x * place.quota ? 0 : 1)) * ROWS * (D + 2);
+        const bool whole = it.all_mine();
+        float *part = P.parts + it.slot_of(blockIdx.x) * ROWS * (D + 2);
         for (int i = tid; i < rows * (D / 4); i += kThreads) {
             const int r = i / (D / 4), d = (i % (D / 4)) * 4;
             float M = s_m[0][r];
@@ -579,7 +498,7 @@ __global__ void __launch_bounds__(kThreads) paged_decode_kernel(const __grid_con
                 const float y[4] = {v.x * inv, v.y * inv, v.z * inv, v.w * inv};
                 ElVec<T, 4> ov;
                 ov.set(y);
-                ov.store((T *)A.out + (long long)(q.q0 + r / G) * A.out_stride + (long long)(head * G + r % G) * D + d);
+                ov.store((T *)A.out + row_at(r, A.out_stride) + d);
             } else {
                 *reinterpret_cast<float4 *>(part + r * D + d) = v;
                 if (d == 0) part[ROWS * D + r] = M, part[ROWS * D + ROWS + r] = L;
@@ -587,17 +506,14 @@ __global__ void __launch_bounds__(kThreads) paged_decode_kernel(const __grid_con
         }
         if (!whole) {
             // ---- the item's parts from CTAs c0 .. c1; the last to arrive joins them in order
-            const long long quota = place.quota;
-            const int c0 = (int)(u0 / quota), c1 = (int)((u0 + tiles - 1) / quota);
+            const int c0 = it.first_cta(), c1 = it.last_cta();
             __threadfence();
             __syncthreads();
             if (tid == 0) s_last = atomicAdd(&P.tickets[c0], 1u) == (unsigned)(c1 - c0);
             __syncthreads();
             if (s_last) {  // uniform
                 __threadfence();
-                auto part_of = [&](int cta) {
-                    return P.parts + (2 * (long long)cta + ((long long)cta * quota >= u0 ? 0 : 1)) * ROWS * (D + 2);
-                };
+                auto part_of = [&](int cta) { return P.parts + it.slot_of(cta) * ROWS * (D + 2); };
                 // every row's maximum over the parts (s_m[0]) and sum (s_l[0])
                 for (int r = warp; r < rows; r += kWarps) {
                     float M = -INFINITY;
@@ -648,13 +564,12 @@ __global__ void __launch_bounds__(kThreads) paged_decode_kernel(const __grid_con
                         const float y[4] = {acc[k].x * inv, acc[k].y * inv, acc[k].z * inv, acc[k].w * inv};
                         ElVec<T, 4> ov;
                         ov.set(y);
-                        ov.store((T *)A.out + (long long)(q.q0 + r / G) * A.out_stride + (long long)(head * G + r % G) * D + d);
+                        ov.store((T *)A.out + row_at(r, A.out_stride) + d);
                     }
                 }
                 if (tid == 0) P.tickets[c0] = 0;  // ready for the next call
             }
         }
-        at = u0 + tb;
         __syncthreads();  // shared memory free for the next item
     }
 }
@@ -673,9 +588,13 @@ int launch_decode_t(const PagedAttnArgs &a, cudaStream_t st) {
     P.A = a;
     P.tickets = (unsigned *)a.work;
     P.parts = (float *)((char *)a.work + kSplitTicketBytes);
-    P.min_quota = 2;
+    const int G = a.n_heads / a.n_kv_heads;
+    P.sets = (G + 8 * NB - 1) / (8 * NB);
+    P.g_set = (G + P.sets - 1) / P.sets;
+    P.line = {8 * NB / P.g_set, a.n_kv_heads * P.sets, 2, 0};
     // no more CTAs than there can be tiles
-    const long long most = (long long)a.b.n_seqs * a.n_kv_heads * ((std::max(1, a.b.max_len) + kTile - 1) / kTile);
+    const long long items = (long long)P.line.heads * (a.b.n_seqs + (long long)a.b.n_tokens / P.line.tq);
+    const long long most = items * ((std::max(1, a.b.max_len) + kTile - 1) / kTile);
     const int grid = (int)std::min<long long>({(long long)num_sms() * std::min(occ, 4), most, kSplitMaxCtas});
     k<<<grid, kThreads, 0, st>>>(P);
     TQ_CUDA_TRY(cudaGetLastError());
@@ -683,25 +602,24 @@ int launch_decode_t(const PagedAttnArgs &a, cudaStream_t st) {
 }
 
 template <typename T, typename C>
-int launch_decode_c(const PagedAttnArgs &a, int rows, cudaStream_t st) {
-    if (a.head_dim == 64)
-        return rows <= 8 ? launch_decode_t<T, C, 64, 1>(a, st) : launch_decode_t<T, C, 64, 2>(a, st);
-    return rows <= 8 ? launch_decode_t<T, C, 128, 1>(a, st) : launch_decode_t<T, C, 128, 2>(a, st);
+int launch_decode_c(const PagedAttnArgs &a, cudaStream_t st) {
+    const bool few = (long long)a.b.max_q_len * (a.n_heads / a.n_kv_heads) <= 8;
+    if (a.head_dim == 64) return few ? launch_decode_t<T, C, 64, 1>(a, st) : launch_decode_t<T, C, 64, 2>(a, st);
+    return few ? launch_decode_t<T, C, 128, 1>(a, st) : launch_decode_t<T, C, 128, 2>(a, st);
 }
 
 }  // namespace
 
-size_t paged_decode_work_bytes(int rows, int head_dim) {
+size_t paged_decode_work_bytes(int head_dim) {
     const size_t ctas = std::min(4 * num_sms(), kSplitMaxCtas);
-    return kSplitTicketBytes + 2 * ctas * (rows <= 8 ? 8 : 16) * (size_t)(head_dim + 2) * 4;
+    return kSplitTicketBytes + 2 * ctas * kDecodeRows * (size_t)(head_dim + 2) * 4;
 }
 
-int launch_paged_decode(const PagedAttnArgs &a, int rows, cudaStream_t st) {
+int launch_paged_decode(const PagedAttnArgs &a, cudaStream_t st) {
     if (a.type == TQB200_EL_F32)
-        return a.cache_type == TQB200_EL_F32 ? launch_decode_c<float, float>(a, rows, st)
-                                             : launch_decode_c<float, __half>(a, rows, st);
-    if (a.type == TQB200_EL_F16) return launch_decode_c<__half, __half>(a, rows, st);
-    return launch_decode_c<__nv_bfloat16, __nv_bfloat16>(a, rows, st);
+        return a.cache_type == TQB200_EL_F32 ? launch_decode_c<float, float>(a, st) : launch_decode_c<float, __half>(a, st);
+    if (a.type == TQB200_EL_F16) return launch_decode_c<__half, __half>(a, st);
+    return launch_decode_c<__nv_bfloat16, __nv_bfloat16>(a, st);
 }
 
 }  // namespace tqb200
