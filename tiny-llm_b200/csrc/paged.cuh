@@ -447,6 +447,9 @@ int launch_paged_attention(const PagedAttnArgs &a, cudaStream_t st);
 int launch_paged_decode(const PagedAttnArgs &a, cudaStream_t st);
 size_t paged_decode_work_bytes(int head_dim);
 constexpr int kDecodeRows = 16;
+// The same with a 16-bit cache; blocks of 128 or 256 query rows.
+int launch_paged_chunk(const PagedAttnArgs &a, cudaStream_t st);
+size_t paged_chunk_work_bytes(int head_dim);
 size_t paged_attention_work_bytes(int n_heads, int n_kv_heads, int head_dim);
 
 }  // namespace tqb200

@@ -52,12 +52,17 @@ int launch_any(const PagedAttnArgs &a, cudaStream_t st) {
 
 size_t paged_attention_work_bytes(int n_heads, int n_kv_heads, int head_dim) {
     (void)n_heads, (void)n_kv_heads;
-    return head_dim == 64 || head_dim == 128 ? paged_decode_work_bytes(head_dim) : 16;
+    return head_dim == 64 || head_dim == 128
+               ? std::max(paged_decode_work_bytes(head_dim), paged_chunk_work_bytes(head_dim)) : 16;
 }
 
 int launch_paged_attention(const PagedAttnArgs &a, cudaStream_t st) {
     if (a.b.n_tokens == 0 || a.b.n_seqs == 0 || a.b.max_q_len == 0) return TQB200_OK;
-    if (a.aligned && (a.head_dim == 64 || a.head_dim == 128)) return launch_paged_decode(a, st);
+    if (a.aligned && (a.head_dim == 64 || a.head_dim == 128)) {
+        const long long rows = (long long)a.b.max_q_len * (a.n_heads / a.n_kv_heads);
+        if (a.cache_type != TQB200_EL_F32 && rows > kDecodeRows) return launch_paged_chunk(a, st);
+        return launch_paged_decode(a, st);
+    }
     if (a.type == TQB200_EL_F32)
         return a.cache_type == TQB200_EL_F32 ? launch_any<float, float>(a, st) : launch_any<float, __half>(a, st);
     if (a.type == TQB200_EL_F16) return launch_any<__half, __half>(a, st);
