@@ -248,42 +248,49 @@ __device__ __noinline__ void row_pass(const PagedAttnArgs &A, const T *q, int se
 // that lies in several CTAs is joined by the last of them to arrive, in the order of the line
 // (the result does not depend on who is last).  Such an item's first CTA names its ticket; a
 // CTA leaves at most two parts: of the item that it begins in the middle of (slot 2c) and of
-// the one that it ends in the middle of (slot 2c + 1).  Where the quota is below `whole_below`
-// tiles, joining would cost more than it saves: CTA c then takes the whole of every item that
-// begins in its range.
+// the one that it ends in the middle of (slot 2c + 1).
+// Where joining (worth `join` tiles of work) would cost more than even shares save, the items
+// are taken whole instead, the sequence's last blocks (its longest) first: CTA c of g takes
+// items c, 2g - 1 - c, 2g + c, ...
 constexpr int kSplitMaxCtas = 1024;
 constexpr size_t kSplitTicketBytes = kSplitMaxCtas * 4;  // head of the workspace, zero between calls
 
 struct LineShape {
     int tq, heads;
-    int min_quota, whole_below;
+    int min_quota, join;  // join < 0: never whole
 };
 
-// Sum of floor((a i + b) / m) over 0 <= i < n: lattice points under a line, by exchanging the
-// axes as in Euclid's algorithm (Graham, Knuth, Patashnik, Concrete Mathematics, 3.5).  With
-// a, b < m the line reaches height h = floor((a (n-1) + b) / m); the points (i, y), 1 <= y <= h,
-// under it are, per y, those with i >= (m y - b) / a:  n h - sum_y ceil((m y - b) / a), and
-// ceil((m y - b) / a) = floor((m (y - 1) + m - b + a - 1) / a).
-__device__ inline long long floor_line_sum(long long n, long long a, long long b, long long m) {
+// Sum of floor((a i + b) / m) over 0 <= i < n, a n + b < 2^32: lattice points under a line, by
+// exchanging the axes as in Euclid's algorithm (Graham, Knuth, Patashnik, Concrete
+// Mathematics, 3.5).  With a, b < m the line reaches height h = floor((a (n-1) + b) / m); the
+// points (i, y), 1 <= y <= h, under it are, per y, those with i >= (m y - b) / a:
+// n h - sum_y ceil((m y - b) / a), and ceil((m y - b) / a) = floor((m (y - 1) + m - b + a - 1) / a).
+__device__ inline long long floor_line_sum(uint32_t n, uint32_t a, uint32_t b, uint32_t m) {
     long long sum = 0, sign = 1;
     while (n > 0) {
         if (a >= m || b >= m) {
-            sum += sign * ((a / m) * (n * (n - 1) / 2) + (b / m) * n);
-            a %= m;
-            b %= m;
+            const uint32_t qa = a / m, qb = b / m;
+            sum += sign * ((long long)qa * ((long long)n * (n - 1) / 2) + (long long)qb * n);
+            a -= qa * m;
+            b -= qb * m;
         }
-        const long long h = (a * (n - 1) + b) / m;
+        const uint32_t h = (a * (n - 1) + b) / m;
         if (h == 0) break;
-        sum += sign * n * h;
+        sum += sign * (long long)n * h;
         sign = -sign;
-        const long long b2 = m - b + a - 1;
+        const uint32_t b2 = m - b + a - 1, m2 = a;
         n = h;
         b = b2;
-        const long long m2 = a;
         a = m;
         m = m2;
     }
     return sum;
+}
+
+// a / b, mostly of 32-bit values
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+    if (((a | b) >> 32) == 0) return (uint32_t)a / (uint32_t)b;
+    return a / b;
 }
 
 template <int KT>
@@ -302,8 +309,9 @@ struct Line {
         if (nb > 1) {
             const int p0 = q.len - q.n;
             // the blocks before it: those that end before position 0 have one tile each
-            const int none = p0 < 0 ? min(nb - 1, (int)(-(long long)p0 / tq)) : 0;
-            sum += nb - 1 + floor_line_sum(nb - 1 - none, tq, (long long)p0 + (long long)none * tq + tq - 1, KT);
+            const int none = p0 < 0 ? min(nb - 1, (int)((uint32_t)(-p0) / (uint32_t)tq)) : 0;
+            sum += nb - 1 + floor_line_sum((uint32_t)(nb - 1 - none), (uint32_t)tq,
+                                           (uint32_t)((long long)p0 + (long long)none * tq + tq - 1), KT);
         }
         return sum;
     }
@@ -313,30 +321,27 @@ struct Line {
     SeqInfo q;
     long long quota, at, end, u0;  // tiles: per CTA; the next, the end of the range; the item's first
     int seq, head, b, nb, tiles, ta, tb;
-    bool whole;                     // the items are taken whole
+    bool whole;                     // the items are taken whole: at, end, u0 count items, u0 the sequence's first
 
     __device__ __forceinline__ void enter_seq(const BatchView &B, int s) {
-        seq = s;
-        q = seq_info(B, s);
-        while (!q.ok || q.n == 0) {
-            if (++seq >= B.n_seqs) return;
+        for (seq = s; seq < B.n_seqs; ++seq) {
             q = seq_info(B, seq);
+            if (q.ok && q.n > 0) break;
         }
         head = 0;
         b = 0;
         nb = blocks(q, sh.tq);
         tiles = block_tiles(q, sh.tq, nb, 0);
     }
-    // The item after this one; seq == n_seqs behind the last.
-    __device__ __forceinline__ void step(const BatchView &B) {
-        u0 += tiles;
-        if (++b == nb) {
-            b = 0;
-            if (++head == sh.heads) {
-                if (++seq < B.n_seqs) enter_seq(B, seq);
-                return;
-            }
+    // whole items: the item number `at`
+    __device__ __forceinline__ void seek(const BatchView &B) {
+        while (at < end && at >= u0 + (long long)nb * sh.heads) {
+            u0 += (long long)nb * sh.heads;
+            enter_seq(B, seq + 1);
         }
+        const long long j = at - u0, back = quotient(j, sh.heads);
+        b = nb - 1 - (int)back;
+        head = (int)(j - back * sh.heads);
         tiles = block_tiles(q, sh.tq, nb, b);
     }
     // The present item's part [ta, tb) for this CTA; false: the range is done.
@@ -347,12 +352,28 @@ struct Line {
         return true;
     }
     __device__ __forceinline__ void next(const BatchView &B) {
+        if (whole) {
+            // c, 2g - 1 - c, 2g + c, ...: the steps alternate, together 2g
+            const long long g = gridDim.x, r = at - quotient(at, 2 * g) * 2 * g;
+            at += r < g ? 2 * (g - r) - 1 : 2 * (2 * g - r) - 1;
+            if (at < end) seek(B);
+            return;
+        }
         at = u0 + tiles;
-        step(B);
+        u0 = at;
+        if (at >= end) return;
+        if (++b == nb) {
+            b = 0;
+            if (++head == sh.heads) {
+                enter_seq(B, seq + 1);
+                return;
+            }
+        }
+        tiles = block_tiles(q, sh.tq, nb, b);
     }
     // The CTAs that share the item: the first and the last.
-    __device__ __forceinline__ int first_cta() const { return (int)(u0 / quota); }
-    __device__ __forceinline__ int last_cta() const { return (int)((u0 + tiles - 1) / quota); }
+    __device__ __forceinline__ int first_cta() const { return (int)quotient(u0, quota); }
+    __device__ __forceinline__ int last_cta() const { return (int)quotient(u0 + tiles - 1, quota); }
     __device__ __forceinline__ bool all_mine() const { return ta == 0 && tb == tiles; }
     __device__ __forceinline__ long long slot_of(int cta) const {
         return 2 * (long long)cta + ((long long)cta * quota >= u0 ? 0 : 1);
@@ -362,43 +383,65 @@ struct Line {
     template <int THREADS>
     __device__ void begin(const BatchView &B, const LineShape &shape, int *status) {
         constexpr int WARPS = THREADS / 32;
-        __shared__ long long s_sum[WARPS], s_first;
-        __shared__ int s_seq;
+        __shared__ long long s_tiles[WARPS], s_items[WARPS], s_first, s_ht;
+        __shared__ int s_most[WARPS], s_seq;
         sh = shape;
         const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
         const int per = (B.n_seqs + THREADS - 1) / THREADS;
         const int s0 = min(B.n_seqs, t * per), s1 = min(B.n_seqs, s0 + per);
-        long long mine = 0;
+        long long mine = 0, items = 0, ht = 0;
+        int most = 0;
         for (int s = s0; s < s1; ++s) {
             const SeqInfo i = seq_info(B, s);
             if (!i.ok && blockIdx.x == 0) report(status, TQB200_PAGED_BAD_SEQ);
-            mine += sh.heads * head_tiles(i, sh.tq);
+            if (!i.ok || i.n == 0) continue;
+            ht = head_tiles(i, sh.tq);
+            const int n = blocks(i, sh.tq);
+            mine += sh.heads * ht;
+            items += (long long)sh.heads * n;
+            most = max(most, block_tiles(i, sh.tq, n, n - 1));
         }
-        long long inc = mine;
+        long long inc = mine, inc_i = items;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long u = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += u;
+            const long long u = __shfl_up_sync(0xffffffffu, inc, o), v = __shfl_up_sync(0xffffffffu, inc_i, o);
+            if (lane >= o) inc += u, inc_i += v;
         }
-        if (lane == 31) s_sum[warp] = inc;
+        most = __reduce_max_sync(0xffffffffu, most);
+        if (lane == 31) s_tiles[warp] = inc, s_items[warp] = inc_i, s_most[warp] = most;
         if (t == 0) s_seq = B.n_seqs;
         __syncthreads();
-        long long before = inc - mine, total = 0;
+        long long before = inc - mine, total = 0, before_i = inc_i - items, total_i = 0;
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
-            if (w < warp) before += s_sum[w];
-            total += s_sum[w];
+            if (w < warp) before += s_tiles[w], before_i += s_items[w];
+            total += s_tiles[w];
+            total_i += s_items[w];
+            most = max(most, s_most[w]);
         }
-        quota = max((total + gridDim.x - 1) / gridDim.x, (long long)sh.min_quota);
-        whole = quota < sh.whole_below;
-        at = blockIdx.x * quota;
-        end = min(at + quota, total);
+        const long long g = gridDim.x;
+        quota = max(quotient(total + g - 1, g), (long long)sh.min_quota);
+        whole = sh.join >= 0 && (total_i <= g ? most : quota + most / 2) <= quota + sh.join;
+        if (whole) {
+            before = before_i, mine = items;
+            at = blockIdx.x;
+            end = total_i;
+        } else {
+            at = blockIdx.x * quota;
+            end = min(at + quota, total);
+        }
         if (at < end && at >= before && at < before + mine) {  // one thread
             for (int s = s0; s < s1; ++s) {
-                const long long n = sh.heads * head_tiles(seq_info(B, s), sh.tq);
+                if (s1 - s0 > 1) ht = head_tiles(seq_info(B, s), sh.tq);
+                long long n = sh.heads * ht;
+                if (whole) {
+                    const SeqInfo i = seq_info(B, s);
+                    n = i.ok ? (long long)sh.heads * blocks(i, sh.tq) : 0;
+                }
                 if (at < before + n) {
                     s_seq = s;
                     s_first = before;
+                    s_ht = ht;
                     break;
                 }
                 before += n;
@@ -410,11 +453,15 @@ struct Line {
             at = end;  // nothing for this CTA
             return;
         }
-        // the item at `at`: head set by division, token block by a scan of 32 blocks at a time
         enter_seq(B, seq);
-        const long long ht = head_tiles(q, sh.tq);
-        head = (int)((at - s_first) / ht);
-        u0 = s_first + head * ht;
+        if (whole) {
+            u0 = s_first;
+            seek(B);
+            return;
+        }
+        // the item at `at`: head set by division, token block by a scan of 32 blocks at a time
+        head = (int)quotient(at - s_first, s_ht);
+        u0 = s_first + head * s_ht;
         long long off = at - u0;
         for (int b0 = 0; b0 < nb; b0 += 32) {
             const int n = b0 + lane < nb ? block_tiles(q, sh.tq, nb, b0 + lane) : 0;
@@ -435,7 +482,6 @@ struct Line {
             off -= __shfl_sync(0xffffffffu, sum, 31);
             u0 += __shfl_sync(0xffffffffu, sum, 31);
         }
-        if (whole && at > u0) next(B);  // begun in the range before
     }
 };
 

@@ -36,9 +36,11 @@ namespace {
 
 constexpr float kRaise = 8.0f;
 constexpr float kLift = 6.0f;
+constexpr int kBehind = 3;        // tiles whose copies a fetching warp leaves in flight
 constexpr int kRows = 128;        // query rows per tile: TMEM lanes
-constexpr int kMaxSlots = 8;
+constexpr int kMaxSlots = 12;
 constexpr int kMarks = 16;        // tiles whose bitmaps are kept (more than the ring holds)
+constexpr int KT = 64;            // positions per tile
 constexpr int kMeta = 1024;
 
 struct ChunkParams {
@@ -85,7 +87,7 @@ __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // 32 columns of this warp's lanes, 32 (fp32 words) or 16 registers a thread
-__device__ __forceinline__ void tm_ld32(uint32_t a, float (&v)[32]) {
+__device__ __forceinline__ void tm_ld32(uint32_t a, float *v) {
     uint32_t r[32];
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
@@ -99,18 +101,16 @@ __device__ __forceinline__ void tm_ld32(uint32_t a, float (&v)[32]) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
-__device__ __forceinline__ void tm_st32(uint32_t a, const float (&v)[32]) {
-    uint32_t r[32];
-#pragma unroll
-    for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(v[i]);
+__device__ __forceinline__ void tm_ld16(uint32_t a, float (&v)[16]) {
+    uint32_t r[16];
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(a),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(a)
         : "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 __device__ __forceinline__ void tm_st16(uint32_t a, const uint32_t (&r)[16]) {
     asm volatile(
@@ -120,6 +120,43 @@ __device__ __forceinline__ void tm_st16(uint32_t a, const uint32_t (&r)[16]) {
         : "memory");
 }
 
+__device__ __forceinline__ void tm_st16(uint32_t a, const float (&v)[16]) {
+    uint32_t r[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(v[i]);
+    tm_st16(a, r);
+}
+
+// two fp32 in one register pair: one instruction for both
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    return v;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float &a, float &b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float v;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(a), "f"(b), "f"(c));
+    return v;
+}
+
+__device__ __forceinline__ bool elect_one() {
+    uint32_t e;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(e));
+    return e != 0;
+}
 __device__ __forceinline__ void arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
@@ -156,27 +193,26 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t 
     lo = *reinterpret_cast<const uint32_t *>(&l);
 }
 
-template <typename T, int D, int QT, int KT>
+template <typename T, int D, int QT>
 struct ChunkShape {
     static constexpr int QS = std::is_same<T, float>::value ? 2 : 1;
     static constexpr int SOFT = QT * 128;                       // softmax threads
     static constexpr int FETCH = 2 * QT;                        // warps that fetch
-    // whole groups of 4 warps; 16 warps per SM either way: 128 registers a thread at launch
-    static constexpr int THREADS = 256 * QT;
+    static constexpr int THREADS = SOFT + FETCH * 32 + QT * 32;  // 14 warps per SM: 128 registers a thread
     static constexpr int ROWS = QT * kRows;
     static constexpr uint32_t QBYTES = kRows * D * 2;           // one operand of one query tile
     static constexpr uint32_t TBYTES = KT * D * 2;              // one slot: a K or a V tile
-    static constexpr uint32_t COLS = QT * (KT + D) <= 256 ? 256 : 512;  // TMEM columns
+    static constexpr uint32_t COLS = QT * (2 * KT + D) <= 256 ? 256 : 512;  // TMEM columns
     // per SM: two where the queries leave room for it
     static constexpr int CTAS = QT == 1 && QS * QBYTES <= 32768 ? 2 : 1;
-    static_assert(QT * (KT + D) <= 512, "TMEM");
+    static_assert(QT * (2 * KT + D) <= 512, "TMEM");
 };
 
 // ---------------------------------------------------------------- the kernel
-template <typename T, typename C, int D, int QT, int KT>
-__global__ void __launch_bounds__(ChunkShape<T, D, QT, KT>::THREADS, ChunkShape<T, D, QT, KT>::CTAS)
+template <typename T, typename C, int D, int QT>
+__global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, ChunkShape<T, D, QT>::CTAS)
     paged_chunk_kernel(const __grid_constant__ ChunkParams P) {
-    using Sh = ChunkShape<T, D, QT, KT>;
+    using Sh = ChunkShape<T, D, QT>;
     constexpr int QS = Sh::QS, ROWS = Sh::ROWS;
     constexpr uint32_t LINE8 = D / 8 * 128;  // bytes of 8 positions (or query rows)
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -184,14 +220,14 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT, KT>::THREADS, ChunkShape<
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     uint64_t *full = reinterpret_cast<uint64_t *>(smem);   // [slots] tile landed (every fetch warp)
     uint64_t *empty = full + kMaxSlots;                    // [slots] tile read by every query tile's products
-    uint64_t *sfull = empty + kMaxSlots;                   // [QT] scores in TMEM
-    uint64_t *pready = sfull + QT;                         // [QT] weights in TMEM (4 warps)
-    uint64_t *odone = pready + QT;                         // [QT] P V complete
-    uint64_t *qready = odone + QT;                         // [QT] queries in shared memory, O free (4 warps)
+    uint64_t *sfull = empty + kMaxSlots;                   // [QT][2] scores in TMEM
+    uint64_t *pready = sfull + 2 * QT;                     // [QT][2] weights in TMEM (4 warps)
+    uint64_t *odone = pready + 2 * QT;                     // [QT][2] P V complete
+    uint64_t *qready = odone + 2 * QT;                       // [QT] queries in shared memory, O free (4 warps)
     uint64_t *done = qready + QT;                          // [QT] every product of the issuing warp complete
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(done + QT);
     uint8_t *marks = smem + 512;                           // [kMarks][KT / 8]: positions that exist
-    static_assert(kMarks * KT / 8 <= kMeta - 512, "marks");
+    static_assert(kMarks * KT / 8 <= kMeta - 512 && 8 * (2 * kMaxSlots + 8 * QT) + 4 <= 512, "meta");
     uint8_t *sq = smem + kMeta;
     uint8_t *ring = sq + QT * QS * Sh::QBYTES;
     __shared__ int s_err;
@@ -202,17 +238,19 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT, KT>::THREADS, ChunkShape<
             mbar_init(&full[i], Sh::FETCH);
             mbar_init(&empty[i], QT);
         }
-        for (int i = 0; i < QT; ++i) {
+        for (int i = 0; i < 2 * QT; ++i) {
             mbar_init(&sfull[i], 1);
             mbar_init(&pready[i], 4);
             mbar_init(&odone[i], 1);
+        }
+        for (int i = 0; i < QT; ++i) {
             mbar_init(&qready[i], 4);
             mbar_init(&done[i], 1);
         }
         fence_mbar_init();
         s_err = 0;
     }
-    Line<KT> it;
+    Line<KT> it{};
     it.template begin<Sh::THREADS>(A.b, P.line, A.status);
     if (it.at >= it.end) return;  // uniform: nothing allocated yet
     constexpr int kIssue = Sh::SOFT / 32 + Sh::FETCH;  // first issuing warp
@@ -234,15 +272,18 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT, KT>::THREADS, ChunkShape<
             if (lane == 0) s_err = 1;
         }
     };
-    uint32_t tiles_done = 0;  // of this CTA, over all its items: phase of the per-tile barriers
+    // Tiles of this CTA so far, over all its items.  Tile n uses the second of each pair of
+    // barriers when n is odd, in their phase n / 2: the softmax runs up to two tiles ahead of
+    // the products, and a parity tells only one phase from the next.
+    uint32_t tiles_done = 0;
     uint32_t items_done = 0;
 
     if (warp < 4 * QT) {
         // ================================================================ softmax
-        if constexpr (QT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");  // 8 x 184 + 8 x 72 = 16 x 128
         const int qt = warp >> 2, r = tid & 127;
+        auto wait_product = [&](uint32_t n) { wait(&odone[2 * qt + (n & 1u)], (n >> 1) & 1u); };
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-        const uint32_t s_at = tmem + lanes + (uint32_t)(qt * KT), o_at = tmem + lanes + (uint32_t)(QT * KT + qt * D);
+        const uint32_t s_of = tmem + lanes + (uint32_t)(qt * 2 * KT), o_at = tmem + lanes + (uint32_t)(QT * 2 * KT + qt * D);
         for (; it.part(A.b); it.next(A.b), ++items_done) {
             const SeqInfo &q = it.q;
             const int head = it.head / P.sets, h0 = (it.head - head * P.sets) * P.g_set;
@@ -251,47 +292,64 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT, KT>::THREADS, ChunkShape<
             const int p0 = q.len - q.n + tok0;
             const int row = qt * kRows + r;
             const bool live = row < rows;
-            const int tok = row / gs;
+            // row / gs for row < 256: error of the reciprocal below 256 * 255 / 65536 < 1
+            const uint32_t recip = (65535u + (uint32_t)gs) / (uint32_t)gs;
+            auto token_of = [&](int x) { return (int)(((uint32_t)x * recip) >> 16); };
+            const int tok = token_of(row);
             const long long q_row = (long long)(q.q0 + tok0 + tok);
             const long long h_off = (long long)(head * G + h0 + row - tok * gs) * D;
             const int see = live ? p0 + tok : -1;
             float c = A.scale * kLog2e;
-            // ---- the row to shared memory
+            // ---- the warp's 32 rows to shared memory: lane (g, j) = (lane / 8, lane % 8) takes the
+            // 16-byte pieces g, g + 4, ... of rows j, j + 8, ... (8 pieces are adjacent there)
             {
-                uint8_t *dst = sq + qt * QS * Sh::QBYTES + (r >> 3) * LINE8 + (r & 7) * 16;
-                const T *src = (const T *)A.q + q_row * A.q_stride + h_off;
-                if constexpr (QS == 1) {
+                const int g = lane >> 3, j = lane & 7;
+                uint8_t *dst0 = sq + qt * QS * Sh::QBYTES + (warp & 3) * 4 * LINE8 + j * 16 + g * 128;
+#pragma unroll 1
+                for (int i = 0; i < 4; ++i) {
+                    const int x = qt * kRows + 32 * (warp & 3) + 8 * i + j, tx = token_of(x);
+                    const bool has = x < rows;
+                    const T *src = (const T *)A.q + (long long)(q.q0 + tok0 + tx) * A.q_stride +
+                                   (long long)(head * G + h0 + x - tx * gs) * D + g * 8;
+                    uint8_t *dst = dst0 + i * LINE8;
+                    if constexpr (QS == 1) {
+                        uint4 v[D / 32];
 #pragma unroll
-                    for (int j = 0; j < D / 8; ++j)
-                        *reinterpret_cast<uint4 *>(dst + j * 128) =
-                            live ? *reinterpret_cast<const uint4 *>(src + j * 8) : make_uint4(0, 0, 0, 0);
-                } else {
-                    float most = 0.0f;
-                    if (live) {
-#pragma unroll 8
-                        for (int j = 0; j < D / 4; ++j) {
-                            const float4 f = *reinterpret_cast<const float4 *>(src + j * 4);
-                            most = fmaxf(most, fmaxf(fmaxf(fabsf(f.x), fabsf(f.y)), fmaxf(fabsf(f.z), fabsf(f.w))));
+                        for (int k = 0; k < D / 32; ++k)
+                            v[k] = has ? *reinterpret_cast<const uint4 *>(src + k * 32) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                        for (int k = 0; k < D / 32; ++k) *reinterpret_cast<uint4 *>(dst + k * 512) = v[k];
+                    } else {
+                        float4 v[D / 32][2];
+                        float most = 0.0f;
+#pragma unroll
+                        for (int k = 0; k < D / 32; ++k)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h)
+                                v[k][h] = has ? *reinterpret_cast<const float4 *>(src + k * 32 + h * 4) : make_float4(0, 0, 0, 0);
+#pragma unroll
+                        for (int k = 0; k < D / 32; ++k)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h)
+                                most = fmaxf(most, fmaxf(fmaxf(fabsf(v[k][h].x), fabsf(v[k][h].y)),
+                                                         fmaxf(fabsf(v[k][h].z), fabsf(v[k][h].w))));
+                        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 8));
+                        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16));
+                        // the row's largest value goes to [2^13, 2^14)
+                        const int e = max(14, min(254, (int)(__float_as_uint(most) >> 23)));
+                        const float up = __uint_as_float((uint32_t)(254 + 13 - e) << 23);
+                        const float mine = __shfl_sync(0xffffffffu, up, j);  // of row 8 i + j
+                        if (g == i) c = c / mine;
+#pragma unroll
+                        for (int k = 0; k < D / 32; ++k) {
+                            uint4 hi, lo;
+                            split2(v[k][0].x * up, v[k][0].y * up, hi.x, lo.x);
+                            split2(v[k][0].z * up, v[k][0].w * up, hi.y, lo.y);
+                            split2(v[k][1].x * up, v[k][1].y * up, hi.z, lo.z);
+                            split2(v[k][1].z * up, v[k][1].w * up, hi.w, lo.w);
+                            *reinterpret_cast<uint4 *>(dst + k * 512) = hi;
+                            *reinterpret_cast<uint4 *>(dst + Sh::QBYTES + k * 512) = lo;
                         }
-                    }
-                    // the row's largest value goes to [2^13, 2^14)
-                    const int e = max(14, min(254, (int)(__float_as_uint(most) >> 23)));
-                    const float up = __uint_as_float((uint32_t)(254 + 13 - e) << 23);
-                    c = c / up;
-#pragma unroll 4
-                    for (int j = 0; j < D / 8; ++j) {
-                        float4 f = make_float4(0, 0, 0, 0), h = f;
-                        if (live) {
-                            f = *reinterpret_cast<const float4 *>(src + j * 8);
-                            h = *reinterpret_cast<const float4 *>(src + j * 8 + 4);
-                        }
-                        uint4 hi, lo;
-                        split2(f.x * up, f.y * up, hi.x, lo.x);
-                        split2(f.z * up, f.w * up, hi.y, lo.y);
-                        split2(h.x * up, h.y * up, hi.z, lo.z);
-                        split2(h.z * up, h.w * up, hi.w, lo.w);
-                        *reinterpret_cast<uint4 *>(dst + j * 128) = hi;
-                        *reinterpret_cast<uint4 *>(dst + Sh::QBYTES + j * 128) = lo;
                     }
                 }
                 fence_proxy_async_smem();
@@ -301,8 +359,9 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT, KT>::THREADS, ChunkShape<
             }
             float m = -INFINITY, l = 0.0f;
             for (int tile = it.ta; tile < it.tb; ++tile, ++tiles_done) {
-                const uint32_t ph = tiles_done & 1u;
-                wait(&sfull[qt], ph);
+                const int buf = tiles_done & 1;
+                const uint32_t s_at = s_of + (uint32_t)(buf * KT);
+                wait(&sfull[2 * qt + buf], (tiles_done >> 1) & 1u);
                 fence_after();
                 // ---- which of the tile's positions the row sees: bit k of word w is position 32 w + k
                 uint32_t vis[KT / 32];
@@ -317,79 +376,70 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT, KT>::THREADS, ChunkShape<
                     }
                     all = __all_sync(0xffffffffu, all);
                 }
-                // ---- the row's maximum
-                float mx = -INFINITY;
+                // ---- the row's scores and their maximum
+                float s[KT];
 #pragma unroll
-                for (int w = 0; w < KT / 32; ++w) {
-                    float s[32];
-                    tm_ld32(s_at + 32 * w, s);
-                    wait_ld();
-                    float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    if (all) {
+                for (int w = 0; w < KT / 32; ++w) tm_ld32(s_at + 32 * w, s + 32 * w);
+                wait_ld();
+                if (!all) {
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) m4[k & 3] = fmaxf(m4[k & 3], s[k]);
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) m4[k & 3] = fmaxf(m4[k & 3], (vis[w] >> k) & 1u ? s[k] : -INFINITY);
-                    }
-                    mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+                    for (int k = 0; k < KT; ++k) s[k] = (vis[k / 32] >> (k & 31)) & 1u ? s[k] : -INFINITY;
                 }
-                mx *= c;
+                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int k = 0; k < KT; k += 2) m4[(k / 2) & 3] = max3(m4[(k / 2) & 3], s[k], s[k + 1]);
+                const float mx = fmaxf(max3(m4[0], m4[1], m4[2]), m4[3]) * c;
                 const bool raise = mx > m + kRaise;
                 if (__any_sync(0xffffffffu, raise)) {
                     const float f = raise ? ex2(m - mx) : 1.0f;  // 0 from -inf
                     if (raise) m = mx;
                     l *= f;
                     if (tile > it.ta) {  // O holds something, once the product before is complete
-                        wait(&odone[qt], ph ^ 1u);
+                        wait_product(tiles_done - 1);
                         fence_after();
-#pragma unroll
-                        for (int d = 0; d < D; d += 32) {
-                            float o[32];
-                            tm_ld32(o_at + d, o);
+#pragma unroll 1
+                        for (int d = 0; d < D; d += 16) {
+                            float o[16];
+                            tm_ld16(o_at + d, o);
                             wait_ld();
 #pragma unroll
-                            for (int k = 0; k < 32; ++k) o[k] *= f;
-                            tm_st32(o_at + d, o);
+                            for (int k = 0; k < 16; ++k) o[k] *= f;
+                            tm_st16(o_at + d, o);
                         }
                     }
                 }
                 // ---- weights, over the scores
                 const float base = m == -INFINITY ? 0.0f : kLift - m;
-                float sum4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                const uint64_t c2 = pair(c, c), base2 = pair(base, base);
+                uint64_t sum2[2] = {pair(0.0f, 0.0f), pair(0.0f, 0.0f)};
 #pragma unroll
                 for (int w = 0; w < KT / 32; ++w) {
-                    float s[32];
-                    tm_ld32(s_at + 32 * w, s);
-                    wait_ld();
+                    uint32_t hi[16], lo[16];
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) s[k] = ex2(fmaf(s[k], c, base));
-                    if (!all) {
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) s[k] = (vis[w] >> k) & 1u ? s[k] : 0.0f;
-                    }
-#pragma unroll
-                    for (int k = 0; k < 32; ++k) sum4[k & 3] += s[k];
-                    uint32_t hi[16];
-                    if constexpr (QS == 1) {
-#pragma unroll
-                        for (int k = 0; k < 16; ++k) hi[k] = pack2<C>(s[2 * k], s[2 * k + 1]);
-                    } else {
-                        uint32_t lo[16];
-#pragma unroll
-                        for (int k = 0; k < 16; ++k) split2(s[2 * k], s[2 * k + 1], hi[k], lo[k]);
-                        tm_st16(s_at + 32 * w + 16, lo);
+                    for (int k = 0; k < 16; ++k) {
+                        float a, b;
+                        unpair(fma2(pair(s[32 * w + 2 * k], s[32 * w + 2 * k + 1]), c2, base2), a, b);
+                        a = ex2(a);
+                        b = ex2(b);
+                        sum2[k & 1] = add2(sum2[k & 1], pair(a, b));
+                        if constexpr (QS == 1) hi[k] = pack2<C>(a, b);
+                        else split2(a, b, hi[k], lo[k]);
                     }
                     tm_st16(s_at + 32 * w, hi);
+                    if constexpr (QS == 2) tm_st16(s_at + 32 * w + 16, lo);
                 }
-                l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
+                {
+                    float a, b;
+                    unpair(add2(sum2[0], sum2[1]), a, b);
+                    l += a + b;
+                }
                 wait_st();
                 fence_before();
                 __syncwarp();
-                if (lane == 0) arrive(&pready[qt]);
+                if (lane == 0) arrive(&pready[2 * qt + buf]);
             }
             // ---- the item's end: O of this part
-            wait(&odone[qt], (tiles_done - 1) & 1u);
+            wait_product(tiles_done - 1);
             fence_after();
             const bool whole = it.all_mine();
             float *part = P.parts + it.slot_of(blockIdx.x) * ROWS * (D + 2);
@@ -498,7 +548,6 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT, KT>::THREADS, ChunkShape<
         }
     } else if (warp < kIssue) {
         // ================================================================ keys and values
-        if constexpr (QT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         const int fw = warp - 4 * QT;
         constexpr int GRP = KT / 8 / Sh::FETCH;     // groups of 8 positions per warp
         const uint32_t ring0 = smem_u32(ring);
@@ -517,14 +566,15 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT, KT>::THREADS, ChunkShape<
             const int head = it.head / P.sets, len = it.q.len;
             const int *table = A.b.table + (long long)it.seq * A.b.table_stride;
             auto place_of = [&](int tile, int i) { return tile * KT + (fw * GRP + i) * 8 + (lane & 7); };
-            int page[GRP];
+            int page[GRP];           // of the next tile's positions, read ahead
+            auto read_pages = [&](int tile) {
 #pragma unroll
-            for (int i = 0; i < GRP; ++i) {
-                const int x = place_of(it.ta, i);
-                page[i] = x < len ? __ldg(table + A.kv.page.div((uint32_t)x)) : -1;
-            }
-            for (int tile = it.ta; tile < it.tb; ++tile, ++tiles_done) {
-                long long off[GRP];
+                for (int i = 0; i < GRP; ++i) {
+                    const int x = place_of(tile, i);
+                    page[i] = tile < it.tb && x < len ? __ldg(table + A.kv.page.div((uint32_t)x)) : -1;
+                }
+            };
+            auto offsets = [&](int tile, long long (&off)[GRP]) {  // of the lane's first piece; -1: none
 #pragma unroll
                 for (int i = 0; i < GRP; ++i) {
                     const int x = place_of(tile, i);
@@ -540,36 +590,47 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT, KT>::THREADS, ChunkShape<
                     }
                     const unsigned have = __ballot_sync(0xffffffffu, off[i] >= 0);
                     if (lane == 0) marks[(tiles_done % kMarks) * (KT / 8) + fw * GRP + i] = (uint8_t)have;
-                    const int xn = place_of(tile + 1, i);
-                    page[i] = tile + 1 < it.tb && xn < len ? __ldg(table + A.kv.page.div((uint32_t)xn)) : -1;
                 }
-#pragma unroll
-                for (int kv = 0; kv < 2; ++kv) {
-                    if (lap > 0 && !bad) {
-                        const uint32_t par = (lap - 1) & 1u;
-                        if (!__all_sync(0xffffffffu, test_once(&empty[slot], par))) {
-                            copies_left<0>();
-                            while (pending > 0) announce();
-                            wait(&empty[slot], par);
-                        }
+                ++tiles_done;
+            };
+            auto fetch = [&](const char *base, const long long (&off)[GRP]) {
+                if (lap > 0 && !bad) {
+                    const uint32_t par = (lap - 1) & 1u;
+                    if (!__all_sync(0xffffffffu, test_once(&empty[slot], par))) {
+                        copies_left<0>();
+                        while (pending > 0) announce();
+                        wait(&empty[slot], par);
                     }
-                    if (!bad) {
-                        const char *base = kv ? A.kv.v : A.kv.k;
-                        const uint32_t dst = ring0 + (uint32_t)slot * Sh::TBYTES + my;
-#pragma unroll
-                        for (int i = 0; i < GRP; ++i)
-#pragma unroll
-                            for (int j = 0; j < D / 32; ++j)
-                                copy16(dst + i * LINE8 + j * 512, off[i] >= 0 ? base + off[i] + j * 64 : base, off[i] >= 0);
-                        asm volatile("cp.async.commit_group;" ::: "memory");
-                        ++pending;
-                        if (pending > 2) {
-                            copies_left<2>();
-                            announce();
-                        }
-                    }
-                    if (++slot == P.slots) slot = 0, ++lap;
                 }
+                if (!bad) {
+                    const uint32_t dst = ring0 + (uint32_t)slot * Sh::TBYTES + my;
+#pragma unroll
+                    for (int i = 0; i < GRP; ++i)
+#pragma unroll
+                        for (int j = 0; j < D / 32; ++j)
+                            copy16(dst + i * LINE8 + j * 512, off[i] >= 0 ? base + off[i] + j * 64 : base, off[i] >= 0);
+                    asm volatile("cp.async.commit_group;" ::: "memory");
+                    if (++pending > kBehind) {
+                        copies_left<kBehind>();
+                        announce();
+                    }
+                }
+                if (++slot == P.slots) slot = 0, ++lap;
+            };
+            long long off[GRP], ahead[GRP] = {};
+            read_pages(it.ta);
+            offsets(it.ta, off);
+            read_pages(it.ta + 1);
+            fetch(A.kv.k, off);
+            for (int tile = it.ta; tile < it.tb; ++tile) {
+                if (tile + 1 < it.tb) {
+                    offsets(tile + 1, ahead);
+                    read_pages(tile + 2);
+                    fetch(A.kv.k, ahead);
+                }
+                fetch(A.kv.v, off);
+#pragma unroll
+                for (int i = 0; i < GRP; ++i) off[i] = ahead[i];
             }
         }
         copies_left<0>();
@@ -577,55 +638,77 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT, KT>::THREADS, ChunkShape<
         if (__any_sync(0xffffffffu, bad_page) && lane == 0) report(A.status, TQB200_PAGED_BAD_PAGE);
     } else {
         // ================================================================ products of query tile qt
-        if constexpr (QT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        const int qt = warp - kIssue;
-        const uint32_t s_at = tmem + (uint32_t)(qt * KT), o_at = tmem + (uint32_t)(QT * KT + qt * D);
-        const uint32_t q_at = smem_u32(sq) + qt * QS * Sh::QBYTES, ring0 = smem_u32(ring);
+        // Every operand of an MMA is made warp-uniform (by shuffles) and one elected lane issues:
+        // 64 clocks per 128 x 128 x 16 product, the pipe's own rate; from a branch on the lane
+        // number, with the descriptors in per-thread registers, each took 96 to 130.
+        auto uniform = [](uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); };
+        const int qt = (int)uniform((uint32_t)(warp - kIssue));
+        const bool one = elect_one();
+        const uint32_t s_of = uniform(tmem) + (uint32_t)(qt * 2 * KT), o_at = uniform(tmem) + (uint32_t)(QT * 2 * KT + qt * D);
+        const uint32_t q_at = uniform(smem_u32(sq)) + qt * QS * Sh::QBYTES, ring0 = uniform(smem_u32(ring));
         constexpr uint32_t id_qk = idesc_of<C>(KT, false), id_pv = idesc_of<C>(D, true);
         int slot = 0;
-        uint32_t lap = 0;
-        auto advance = [&]() {
-            if (++slot == P.slots) slot = 0, ++lap;
-        };
-        for (; qt < QT && it.part(A.b); it.next(A.b), ++items_done) {
-            wait(&qready[qt], items_done & 1u);
-            for (int tile = it.ta; tile < it.tb; ++tile, ++tiles_done) {
-                // scores; the slots of K and V alternate, so K of the next tile follows V of this one
-                wait(&full[slot], lap & 1u);
-                if (!bad && lane == 0) {
-                    fence_after();
-                    const uint32_t k_at = ring0 + (uint32_t)slot * Sh::TBYTES;
+        uint32_t lap = 0, scored = 0;  // tiles whose scores were issued
+        // S[scored % 2] = Q K^T of the next K slot
+        auto scores = [&]() {
+            wait(&full[slot], lap & 1u);
+            if (!bad) {
+                fence_after();
+                const uint64_t qd = core_desc(q_at, 128, LINE8);
+                const uint64_t kd = core_desc(uniform(ring0 + (uint32_t)slot * Sh::TBYTES), 128, LINE8);
+                const int buf = (int)uniform(scored & 1u);
+                if (one) {
 #pragma unroll
                     for (int ks = 0; ks < D / 16; ++ks)
 #pragma unroll
                         for (int sp = QS - 1; sp >= 0; --sp)
-                            mma_ss(s_at, core_desc(q_at + sp * Sh::QBYTES + ks * 256, 128, LINE8),
-                                   core_desc(k_at + ks * 256, 128, LINE8), id_qk, ks > 0 || sp < QS - 1);
-                    mma_commit(&sfull[qt]);
+                            mma_ss(s_of + buf * KT, qd + (sp * Sh::QBYTES + ks * 256) / 16, kd + ks * 16, id_qk,
+                                   ks > 0 || sp < QS - 1);
+                    mma_commit(&sfull[2 * qt + buf]);
                     mma_commit(&empty[slot]);
                 }
-                __syncwarp();
-                advance();
-                wait(&pready[qt], tiles_done & 1u);
+            }
+            __syncwarp();
+            ++scored;
+            if (++slot == P.slots) slot = 0, ++lap;
+        };
+        auto wait_product = [&](uint32_t n) { wait(&odone[2 * qt + (n & 1u)], (n >> 1) & 1u); };
+        for (; qt < QT && it.part(A.b); it.next(A.b), ++items_done) {
+            wait(&qready[qt], items_done & 1u);
+            scores();
+            for (int tile = it.ta; tile < it.tb; ++tile, ++tiles_done) {
+                if (tile + 1 < it.tb) {
+                    // The buffer holds the weights of the tile before: the product that reads
+                    // them has another shape than this one, and only products of one shape and
+                    // accumulator are ordered by their issue, so its end is waited for.
+                    if (tile > it.ta) wait_product(tiles_done - 1);
+                    scores();  // runs while the softmax of this tile does
+                }
+                const int buf = (int)uniform(tiles_done & 1u);
+                wait(&pready[2 * qt + buf], (tiles_done >> 1) & 1u);
                 wait(&full[slot], lap & 1u);
-                if (!bad && lane == 0) {
+                if (!bad) {
                     fence_after();
-                    const uint32_t v_at = ring0 + (uint32_t)slot * Sh::TBYTES;
+                    const uint64_t vd = core_desc(uniform(ring0 + (uint32_t)slot * Sh::TBYTES), LINE8, 128);
+                    const bool more = uniform(tile > it.ta) != 0;
+                    const uint32_t p_at = s_of + buf * KT;
+                    if (one) {
 #pragma unroll
-                    for (int kk = 0; kk < KT / 16; ++kk)
+                        for (int kk = 0; kk < KT / 16; ++kk)
 #pragma unroll
-                        for (int sp = QS - 1; sp >= 0; --sp)
-                            mma_ts(o_at, s_at + 32 * (kk >> 1) + 8 * (kk & 1) + 16 * sp,
-                                   core_desc(v_at + kk * 2 * LINE8, LINE8, 128), id_pv, tile > it.ta || kk > 0 || sp < QS - 1);
-                    mma_commit(&odone[qt]);
-                    mma_commit(&empty[slot]);
+                            for (int sp = QS - 1; sp >= 0; --sp)
+                                mma_ts(o_at, p_at + 32 * (kk >> 1) + 8 * (kk & 1) + 16 * sp, vd + kk * 2 * (LINE8 / 16), id_pv,
+                                       kk > 0 || sp < QS - 1 || more);
+                        mma_commit(&odone[2 * qt + buf]);
+                        mma_commit(&empty[slot]);
+                    }
                 }
                 __syncwarp();
-                advance();
+                if (++slot == P.slots) slot = 0, ++lap;
             }
         }
-        if (qt < QT && lane == 0) {  // everything issued above is complete before shared memory and TMEM go
-            mma_commit(&done[qt]);
+        if (qt < QT) {  // everything issued above is complete before shared memory and TMEM go
+            if (one) mma_commit(&done[qt]);
             if (!mbar_wait_sleep(&done[qt], 0u, kWaitCycles)) s_err = 1;
         }
         __syncwarp();
@@ -639,17 +722,17 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT, KT>::THREADS, ChunkShape<
     if (tid == 0 && s_err) report(A.status, TQB200_PAGED_TIMEOUT);
 }
 
-template <typename T, typename C, int D, int QT, int KT>
+template <typename T, typename C, int D, int QT>
 int launch_chunk_t(const PagedAttnArgs &a, cudaStream_t st) {
-    using Sh = ChunkShape<T, D, QT, KT>;
-    auto k = paged_chunk_kernel<T, C, D, QT, KT>;
+    using Sh = ChunkShape<T, D, QT>;
+    auto k = paged_chunk_kernel<T, C, D, QT>;
     static KernelSmem once;
     int limit = 0;
     TQ_CUDA_TRY(smem_limit_once(k, once, &limit));
     if (Sh::CTAS == 2) limit = std::min(limit, 112 * 1024);  // of the SM's 228 KB, 1 KB per CTA reserved
     const int fixed = kMeta + QT * Sh::QS * (int)Sh::QBYTES;
     const int slots = std::min(kMaxSlots, (limit - fixed) / (int)Sh::TBYTES);
-    TQ_CHECK_ARG(slots >= 3, "paged_attention: %d bytes of shared memory hold %d tiles", limit, slots);
+    TQ_CHECK_ARG(slots >= kBehind + 1, "paged_attention: %d bytes of shared memory hold %d tiles", limit, slots);
     ChunkParams P{};
     P.A = a;
     P.tickets = (unsigned *)a.work;
@@ -657,7 +740,7 @@ int launch_chunk_t(const PagedAttnArgs &a, cudaStream_t st) {
     const int G = a.n_heads / a.n_kv_heads;
     P.sets = (G + Sh::ROWS - 1) / Sh::ROWS;
     P.g_set = (G + P.sets - 1) / P.sets;
-    P.line = {Sh::ROWS / P.g_set, a.n_kv_heads * P.sets, 1, 8};
+    P.line = {Sh::ROWS / P.g_set, a.n_kv_heads * P.sets, 1, 12};
     P.slots = slots;
     const long long items = (long long)P.line.heads * (a.b.n_seqs + (long long)a.b.n_tokens / P.line.tq);
     const long long most = items * ((std::max(1, a.b.max_len) + KT - 1) / KT);
@@ -669,12 +752,9 @@ int launch_chunk_t(const PagedAttnArgs &a, cudaStream_t st) {
 
 template <typename T, typename C>
 int launch_chunk_c(const PagedAttnArgs &a, cudaStream_t st) {
-    constexpr bool split = std::is_same<T, float>::value;
     const bool big = (long long)a.b.n_tokens * a.n_heads >= 256LL * num_sms();
-    if (a.head_dim == 64)
-        return big ? launch_chunk_t<T, C, 64, 2, 128>(a, st) : launch_chunk_t<T, C, 64, 1, 64>(a, st);
-    if constexpr (split) return big ? launch_chunk_t<T, C, 128, 2, 64>(a, st) : launch_chunk_t<T, C, 128, 1, 64>(a, st);
-    else return big ? launch_chunk_t<T, C, 128, 2, 128>(a, st) : launch_chunk_t<T, C, 128, 1, 64>(a, st);
+    if (a.head_dim == 64) return big ? launch_chunk_t<T, C, 64, 2>(a, st) : launch_chunk_t<T, C, 64, 1>(a, st);
+    return big ? launch_chunk_t<T, C, 128, 2>(a, st) : launch_chunk_t<T, C, 128, 1>(a, st);
 }
 
 }  // namespace
