@@ -249,6 +249,8 @@ __device__ __noinline__ void row_pass(const PagedAttnArgs &A, const T *q, int se
 // (the result does not depend on who is last).  Such an item's first CTA names its ticket; a
 // CTA leaves at most two parts: of the item that it begins in the middle of (slot 2c) and of
 // the one that it ends in the middle of (slot 2c + 1).
+// Beginning an item (its queries, the first tile's latency, its results) costs as much as `over`
+// tiles, so the line counts as many units more at the front of each item.
 // Where joining (worth `join` tiles of work) would cost more than even shares save, the items
 // are taken whole instead, the sequence's last blocks (its longest) first: CTA c of g takes
 // items c, 2g - 1 - c, 2g + c, ...
@@ -257,7 +259,7 @@ constexpr size_t kSplitTicketBytes = kSplitMaxCtas * 4;  // head of the workspac
 
 struct LineShape {
     int tq, heads;
-    int min_quota, join;  // join < 0: never whole
+    int min_quota, over, join;  // join < 0: never whole
 };
 
 // Sum of floor((a i + b) / m) over 0 <= i < n, a n + b < 2^32: lattice points under a line, by
@@ -319,25 +321,31 @@ struct Line {
     // ---- one warp's way along its CTA's part of the line (every warp walks it for itself)
     LineShape sh;
     SeqInfo q;
-    long long quota, at, end, u0;  // tiles: per CTA; the next, the end of the range; the item's first
+    long long quota, at, end, u0;  // units: per CTA; the next, the end of the range; the item's first tile
     int seq, head, b, nb, tiles, ta, tb;
     bool whole;                     // the items are taken whole: at, end, u0 count items, u0 the sequence's first
 
-    __device__ __forceinline__ void enter_seq(const BatchView &B, int s) {
-        for (seq = s; seq < B.n_seqs; ++seq) {
-            q = seq_info(B, seq);
-            if (q.ok && q.n > 0) break;
-        }
+    __device__ __forceinline__ void enter(const SeqInfo &i, int s) {
+        seq = s;
+        q = i;
         head = 0;
         b = 0;
         nb = blocks(q, sh.tq);
         tiles = block_tiles(q, sh.tq, nb, 0);
     }
+    __device__ __forceinline__ void enter_from(const BatchView &B, int s) {
+        SeqInfo i{};
+        for (; s < B.n_seqs; ++s) {
+            i = seq_info(B, s);
+            if (i.ok && i.n > 0) break;
+        }
+        enter(i, s);
+    }
     // whole items: the item number `at`
     __device__ __forceinline__ void seek(const BatchView &B) {
-        while (at < end && at >= u0 + (long long)nb * sh.heads) {
+        while (at < end && at >= u0 + (long long)nb * sh.heads && seq < B.n_seqs) {
             u0 += (long long)nb * sh.heads;
-            enter_seq(B, seq + 1);
+            enter_from(B, seq + 1);
         }
         const long long j = at - u0, back = quotient(j, sh.heads);
         b = nb - 1 - (int)back;
@@ -347,9 +355,9 @@ struct Line {
     // The present item's part [ta, tb) for this CTA; false: the range is done.
     __device__ __forceinline__ bool part(const BatchView &B) {
         if (at >= end || seq >= B.n_seqs) return false;
-        ta = whole ? 0 : (int)(at - u0);
+        ta = whole ? 0 : (int)max(0LL, at - u0);
         tb = whole ? tiles : (int)min((long long)tiles, end - u0);
-        return true;
+        return tb > ta;  // a range may end in the units before an item's first tile
     }
     __device__ __forceinline__ void next(const BatchView &B) {
         if (whole) {
@@ -360,12 +368,12 @@ struct Line {
             return;
         }
         at = u0 + tiles;
-        u0 = at;
+        u0 = at + sh.over;
         if (at >= end) return;
         if (++b == nb) {
             b = 0;
             if (++head == sh.heads) {
-                enter_seq(B, seq + 1);
+                enter_from(B, seq + 1);
                 return;
             }
         }
@@ -379,92 +387,35 @@ struct Line {
         return 2 * (long long)cta + ((long long)cta * quota >= u0 ? 0 : 1);
     }
 
-    // Whole CTA (THREADS of it), once: the line's length, the range, the first item.
-    template <int THREADS>
-    __device__ void begin(const BatchView &B, const LineShape &shape, int *status) {
-        constexpr int WARPS = THREADS / 32;
-        __shared__ long long s_tiles[WARPS], s_items[WARPS], s_first, s_ht;
-        __shared__ int s_most[WARPS], s_seq;
-        sh = shape;
-        const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-        const int per = (B.n_seqs + THREADS - 1) / THREADS;
-        const int s0 = min(B.n_seqs, t * per), s1 = min(B.n_seqs, s0 + per);
-        long long mine = 0, items = 0, ht = 0;
-        int most = 0;
-        for (int s = s0; s < s1; ++s) {
-            const SeqInfo i = seq_info(B, s);
-            if (!i.ok && blockIdx.x == 0) report(status, TQB200_PAGED_BAD_SEQ);
-            if (!i.ok || i.n == 0) continue;
-            ht = head_tiles(i, sh.tq);
-            const int n = blocks(i, sh.tq);
-            mine += sh.heads * ht;
-            items += (long long)sh.heads * n;
-            most = max(most, block_tiles(i, sh.tq, n, n - 1));
-        }
-        long long inc = mine, inc_i = items;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long u = __shfl_up_sync(0xffffffffu, inc, o), v = __shfl_up_sync(0xffffffffu, inc_i, o);
-            if (lane >= o) inc += u, inc_i += v;
-        }
-        most = __reduce_max_sync(0xffffffffu, most);
-        if (lane == 31) s_tiles[warp] = inc, s_items[warp] = inc_i, s_most[warp] = most;
-        if (t == 0) s_seq = B.n_seqs;
-        __syncthreads();
-        long long before = inc - mine, total = 0, before_i = inc_i - items, total_i = 0;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
-            if (w < warp) before += s_tiles[w], before_i += s_items[w];
-            total += s_tiles[w];
-            total_i += s_items[w];
-            most = max(most, s_most[w]);
-        }
+    // The range of CTA blockIdx.x from the line's totals; `before`, `mine`: units of the caller's
+    // sequences and of those before them.  Leaves them as items where items are taken whole.
+    __device__ __forceinline__ void range(long long total, long long items, int most) {
         const long long g = gridDim.x;
         quota = max(quotient(total + g - 1, g), (long long)sh.min_quota);
-        whole = sh.join >= 0 && (total_i <= g ? most : quota + most / 2) <= quota + sh.join;
+        most += sh.over;
+        whole = sh.join >= 0 && (items <= g ? most : quota + most / 2) <= quota + sh.join;
+        at = whole ? (long long)blockIdx.x : blockIdx.x * quota;
+        end = whole ? items : min(at + quota, total);
+    }
+    // Into sequence s, whose units (or items) begin at `first` and whose head sets have `hu` units.
+    __device__ __forceinline__ void locate(const BatchView &B, const SeqInfo &i, int s, long long first, long long hu) {
+        const int lane = threadIdx.x & 31;
+        enter(i, s);
         if (whole) {
-            before = before_i, mine = items;
-            at = blockIdx.x;
-            end = total_i;
-        } else {
-            at = blockIdx.x * quota;
-            end = min(at + quota, total);
-        }
-        if (at < end && at >= before && at < before + mine) {  // one thread
-            for (int s = s0; s < s1; ++s) {
-                if (s1 - s0 > 1) ht = head_tiles(seq_info(B, s), sh.tq);
-                long long n = sh.heads * ht;
-                if (whole) {
-                    const SeqInfo i = seq_info(B, s);
-                    n = i.ok ? (long long)sh.heads * blocks(i, sh.tq) : 0;
-                }
-                if (at < before + n) {
-                    s_seq = s;
-                    s_first = before;
-                    s_ht = ht;
-                    break;
-                }
-                before += n;
-            }
-        }
-        __syncthreads();
-        seq = s_seq;
-        if (at >= end || seq >= B.n_seqs) {
-            at = end;  // nothing for this CTA
-            return;
-        }
-        enter_seq(B, seq);
-        if (whole) {
-            u0 = s_first;
+            u0 = first;
             seek(B);
             return;
         }
-        // the item at `at`: head set by division, token block by a scan of 32 blocks at a time
-        head = (int)quotient(at - s_first, s_ht);
-        u0 = s_first + head * s_ht;
+        // head set by division, token block by a scan of 32 blocks at a time
+        head = (int)quotient(at - first, hu);
+        u0 = first + head * hu;
         long long off = at - u0;
+        if (nb == 1) {
+            u0 += sh.over;
+            return;
+        }
         for (int b0 = 0; b0 < nb; b0 += 32) {
-            const int n = b0 + lane < nb ? block_tiles(q, sh.tq, nb, b0 + lane) : 0;
+            const int n = b0 + lane < nb ? block_tiles(q, sh.tq, nb, b0 + lane) + sh.over : 0;
             int sum = n;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -475,13 +426,120 @@ struct Line {
             if (past) {
                 const int l = __ffs((int)past) - 1;
                 b = b0 + l;
-                tiles = __shfl_sync(0xffffffffu, n, l);
+                tiles = __shfl_sync(0xffffffffu, n, l) - sh.over;
                 u0 += __shfl_sync(0xffffffffu, sum, l) - tiles;
-                break;
+                return;
             }
             off -= __shfl_sync(0xffffffffu, sum, 31);
             u0 += __shfl_sync(0xffffffffu, sum, 31);
         }
+    }
+
+    // Whole CTA (THREADS of it), once: the line's length, the range, the first item.
+    template <int THREADS>
+    __device__ void begin(const BatchView &B, const LineShape &shape, int *status) {
+        sh = shape;
+        const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+        if (B.n_seqs <= 32) {
+            // every warp for itself, a lane per sequence: no barrier, one round of loads
+            SeqInfo i{};
+            if (lane < B.n_seqs) {
+                i = seq_info(B, lane);
+                if (!i.ok && t < 32 && blockIdx.x == 0) report(status, TQB200_PAGED_BAD_SEQ);
+            }
+            const bool has = i.ok && i.n > 0;
+            const int n = has ? blocks(i, sh.tq) : 0;
+            const long long hu = has ? head_tiles(i, sh.tq) + (long long)n * sh.over : 0;
+            const long long mine = hu * sh.heads, mine_i = (long long)n * sh.heads;
+            long long inc = mine, inc_i = mine_i;
+            if (B.n_seqs > 1) {
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const long long u = __shfl_up_sync(0xffffffffu, inc, o), v = __shfl_up_sync(0xffffffffu, inc_i, o);
+                    if (lane >= o) inc += u, inc_i += v;
+                }
+            }
+            const int last = B.n_seqs - 1;
+            const int most = __reduce_max_sync(0xffffffffu, has ? block_tiles(i, sh.tq, n, n - 1) : 0);
+            range(__shfl_sync(0xffffffffu, inc, last), __shfl_sync(0xffffffffu, inc_i, last), most);
+            const unsigned past = __ballot_sync(0xffffffffu, lane < B.n_seqs && at < (whole ? inc_i : inc));
+            seq = B.n_seqs;
+            if (at >= end || past == 0) {
+                at = end;  // nothing for this CTA
+                return;
+            }
+            const int s = __ffs((int)past) - 1;
+            SeqInfo f;
+            f.q0 = __shfl_sync(0xffffffffu, i.q0, s);
+            f.n = __shfl_sync(0xffffffffu, i.n, s);
+            f.len = __shfl_sync(0xffffffffu, i.len, s);
+            f.ok = 1;
+            locate(B, f, s, __shfl_sync(0xffffffffu, whole ? inc_i - mine_i : inc - mine, s), __shfl_sync(0xffffffffu, hu, s));
+            return;
+        }
+        constexpr int WARPS = THREADS / 32;
+        __shared__ long long s_units[WARPS], s_items[WARPS], s_first, s_hu;
+        __shared__ int s_most[WARPS], s_seq;
+        const int per = (B.n_seqs + THREADS - 1) / THREADS;
+        const int s0 = min(B.n_seqs, t * per), s1 = min(B.n_seqs, s0 + per);
+        auto units_of = [&](const SeqInfo &i, long long &hu, long long &items) {
+            items = 0;
+            hu = 0;
+            if (!i.ok || i.n == 0) return;
+            const int n = blocks(i, sh.tq);
+            items = (long long)n * sh.heads;
+            hu = head_tiles(i, sh.tq) + (long long)n * sh.over;
+        };
+        long long mine = 0, mine_i = 0, hu = 0, n = 0;
+        int most = 0;
+        for (int s = s0; s < s1; ++s) {
+            const SeqInfo i = seq_info(B, s);
+            if (!i.ok && blockIdx.x == 0) report(status, TQB200_PAGED_BAD_SEQ);
+            units_of(i, hu, n);
+            mine += hu * sh.heads;
+            mine_i += n;
+            if (n) most = max(most, block_tiles(i, sh.tq, blocks(i, sh.tq), blocks(i, sh.tq) - 1));
+        }
+        long long inc = mine, inc_i = mine_i;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long u = __shfl_up_sync(0xffffffffu, inc, o), v = __shfl_up_sync(0xffffffffu, inc_i, o);
+            if (lane >= o) inc += u, inc_i += v;
+        }
+        most = __reduce_max_sync(0xffffffffu, most);
+        if (lane == 31) s_units[warp] = inc, s_items[warp] = inc_i, s_most[warp] = most;
+        if (t == 0) s_seq = B.n_seqs;
+        __syncthreads();
+        long long before = inc - mine, total = 0, before_i = inc_i - mine_i, total_i = 0;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            if (w < warp) before += s_units[w], before_i += s_items[w];
+            total += s_units[w];
+            total_i += s_items[w];
+            most = max(most, s_most[w]);
+        }
+        range(total, total_i, most);
+        if (whole) before = before_i, mine = mine_i;
+        if (at < end && at >= before && at < before + mine) {  // one thread
+            for (int s = s0; s < s1; ++s) {
+                if (s1 - s0 > 1) units_of(seq_info(B, s), hu, n);
+                const long long u = whole ? n : hu * sh.heads;
+                if (at < before + u) {
+                    s_seq = s;
+                    s_first = before;
+                    s_hu = hu;
+                    break;
+                }
+                before += u;
+            }
+        }
+        __syncthreads();
+        seq = s_seq;
+        if (at >= end || seq >= B.n_seqs) {
+            at = end;  // nothing for this CTA
+            return;
+        }
+        locate(B, seq_info(B, seq), seq, s_first, s_hu);
     }
 };
 

@@ -740,7 +740,7 @@ int launch_chunk_t(const PagedAttnArgs &a, cudaStream_t st) {
     const int G = a.n_heads / a.n_kv_heads;
     P.sets = (G + Sh::ROWS - 1) / Sh::ROWS;
     P.g_set = (G + P.sets - 1) / P.sets;
-    P.line = {Sh::ROWS / P.g_set, a.n_kv_heads * P.sets, 1, 12};
+    P.line = {Sh::ROWS / P.g_set, a.n_kv_heads * P.sets, 1, 4, 10};
     P.slots = slots;
     const long long items = (long long)P.line.heads * (a.b.n_seqs + (long long)a.b.n_tokens / P.line.tq);
     const long long most = items * ((std::max(1, a.b.max_len) + KT - 1) / KT);

@@ -105,8 +105,12 @@ __device__ __forceinline__ uint32_t word(const uint4 &v, int i) { return i == 0 
 
 // ---------------------------------------------------------------- the kernel
 // T activations, C cache, D head_dim, NB blocks of 8 query rows.
+template <typename C, int D, int NB>
+constexpr int kPerSm = D == 64 ? (NB == 1 ? 4 : std::is_same<C, float>::value ? 2 : 3)
+                               : (NB == 1 && !std::is_same<C, float>::value ? 3 : 2);  // CTAs: by registers
+
 template <typename T, typename C, int D, int NB>
-__global__ void __launch_bounds__(kThreads) paged_decode_kernel(const __grid_constant__ DecodeParams P) {
+__global__ void __launch_bounds__(kThreads, kPerSm<C, D, NB>) paged_decode_kernel(const __grid_constant__ DecodeParams P) {
     constexpr bool F32 = std::is_same<C, float>::value;
     constexpr bool SPLIT = !F32 && std::is_same<T, float>::value;  // hi + lo fp16 operands
     constexpr int QS = F32 || SPLIT ? 2 : 1;
@@ -122,11 +126,12 @@ __global__ void __launch_bounds__(kThreads) paged_decode_kernel(const __grid_con
     // one buffer, in turn: the query operands while the item's tiles are read, the warps'
     // accumulators at its end, the weights of up to 128 parts when they are joined
     constexpr size_t kBuf = std::max({sizeof(float) * kWarps * ROWS * D, sizeof(uint4) * QS * NB * KC * 32,
-                                      sizeof(float) * ROWS * kThreads});
+                                      sizeof(float) * 2 * ROWS * kThreads});
     __shared__ __align__(16) char s_buf[kBuf];
     auto &s_o = *reinterpret_cast<float(*)[kWarps][ROWS][D]>(s_buf);
     auto &s_q = *reinterpret_cast<uint4(*)[QS * NB * KC][32]>(s_buf);
     auto &s_w = *reinterpret_cast<float(*)[ROWS][kThreads]>(s_buf);
+    auto &s_p = *reinterpret_cast<float(*)[ROWS][kThreads]>(s_buf + sizeof(float) * ROWS * kThreads);
     __shared__ float s_m[kWarps][ROWS], s_l[kWarps][ROWS];
     __shared__ float s_c[ROWS];
     __shared__ unsigned s_last;
@@ -144,8 +149,11 @@ __global__ void __launch_bounds__(kThreads) paged_decode_kernel(const __grid_con
         const int rows = min(P.line.tq, q.n - tok0) * gs;
         const int p0 = q.len - q.n + tok0;  // position of the first row
         const int *table = A.b.table + (long long)it.seq * A.b.table_stride;
+        const uint32_t recip = (65535u + (uint32_t)gs) / (uint32_t)gs;  // r / gs for r < 256
+        auto token_of = [&](int r) { return (int)(((uint32_t)r * recip) >> 16); };
         auto row_at = [&](int r, long long stride) {
-            return (long long)(q.q0 + tok0 + r / gs) * stride + (long long)(head * G + h0 + r % gs) * D;
+            const int t = token_of(r);
+            return (long long)(q.q0 + tok0 + t) * stride + (long long)(head * G + h0 + r - t * gs) * D;
         };
         auto row_q = [&](int r) {
             return (const T *)A.q + row_at(r, A.q_stride);
@@ -190,6 +198,20 @@ __global__ void __launch_bounds__(kThreads) paged_decode_kernel(const __grid_con
             }
         };
         int page1 = page_of(ta);
+        // the queries' loads go out before the keys', which wait for their pages
+        constexpr int QW = std::is_same<T, float>::value ? EL / 4 : 1;  // 16-byte loads per piece
+        uint4 qraw[NB][KC][QW];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            if (!QREG && warp != (nb & (kWarps - 1))) continue;
+            const int r = 8 * nb + g;
+            const T *src = row_q(min(r, rows - 1)) + t4 * EL;
+#pragma unroll
+            for (int j = 0; j < KC; ++j)
+#pragma unroll
+                for (int e = 0; e < QW; ++e)
+                    qraw[nb][j][e] = r < rows ? *reinterpret_cast<const uint4 *>(src + j * 4 * EL + e * 4) : make_uint4(0, 0, 0, 0);
+        }
         long long off = offset_of(ta, page1);
         page1 = page_of(ta + 1);
         load_k(off);
@@ -206,16 +228,13 @@ __global__ void __launch_bounds__(kThreads) paged_decode_kernel(const __grid_con
             if (QREG || warp == (nb & (kWarps - 1))) {
                 if constexpr (std::is_same<T, float>::value) {
                     float x[KC][EL];
-                    const float *src = r < rows ? row_q(r) + t4 * EL : nullptr;
                     float most = 0.0f;
 #pragma unroll
                     for (int j = 0; j < KC; ++j)
 #pragma unroll
-                        for (int e = 0; e < EL; e += 4) {
-                            const float4 f = src ? *reinterpret_cast<const float4 *>(src + j * 4 * EL + e)
-                                                 : make_float4(0, 0, 0, 0);
-                            x[j][e] = f.x, x[j][e + 1] = f.y, x[j][e + 2] = f.z, x[j][e + 3] = f.w;
-                            most = fmaxf(most, fmaxf(fmaxf(fabsf(f.x), fabsf(f.y)), fmaxf(fabsf(f.z), fabsf(f.w))));
+                        for (int e = 0; e < EL; ++e) {
+                            x[j][e] = __uint_as_float(word(qraw[nb][j][e / 4], e & 3));
+                            most = fmaxf(most, fabsf(x[j][e]));
                         }
                     if constexpr (SPLIT) {
                         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
@@ -245,8 +264,7 @@ __global__ void __launch_bounds__(kThreads) paged_decode_kernel(const __grid_con
                 } else {
 #pragma unroll
                     for (int j = 0; j < KC; ++j) {
-                        const uint4 v = r < rows ? *reinterpret_cast<const uint4 *>(row_q(r) + (t4 + 4 * j) * EL)
-                                                 : make_uint4(0, 0, 0, 0);
+                        const uint4 v = qraw[nb][j][0];
                         if constexpr (QREG) qr[nb * KC + j] = v;
                         else s_q[nb * KC + j][lane] = v;
                     }
@@ -257,7 +275,7 @@ __global__ void __launch_bounds__(kThreads) paged_decode_kernel(const __grid_con
             for (int e = 0; e < 2; ++e) {
                 const int col = 8 * nb + 2 * t4 + e;
                 if (QREG) c[nb][e] = __shfl_sync(0xffffffffu, c_row, (2 * t4 + e) * 4);
-                see[nb][e] = col < rows ? p0 + col / gs : -1;
+                see[nb][e] = col < rows ? p0 + token_of(col) : -1;
             }
         }
         if (!QREG) {
@@ -294,8 +312,9 @@ __global__ void __launch_bounds__(kThreads) paged_decode_kernel(const __grid_con
             float s[NB][4];
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
+                float s2[4];  // a second chain of sums: half the products' latency
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[nb][e] = 0.0f;
+                for (int e = 0; e < 4; ++e) s[nb][e] = s2[e] = 0.0f;
 #pragma unroll
                 for (int j = 0; j < KC; ++j) {
                     if constexpr (F32) {
@@ -307,19 +326,21 @@ __global__ void __launch_bounds__(kThreads) paged_decode_kernel(const __grid_con
                             tf32_split(__uint_as_float(word(kr[1][j], 2 * u)), hi[1], lo[1]);
                             tf32_split(__uint_as_float(word(kr[0][j], 2 * u + 1)), hi[2], lo[2]);
                             tf32_split(__uint_as_float(word(kr[1][j], 2 * u + 1)), hi[3], lo[3]);
-                            mma_tf32(s[nb], lo, word(qh, 2 * u), word(qh, 2 * u + 1));
-                            mma_tf32(s[nb], hi, word(ql, 2 * u), word(ql, 2 * u + 1));
+                            mma_tf32(s2, lo, word(qh, 2 * u), word(qh, 2 * u + 1));
+                            mma_tf32(s2, hi, word(ql, 2 * u), word(ql, 2 * u + 1));
                             mma_tf32(s[nb], hi, word(qh, 2 * u), word(qh, 2 * u + 1));
                         }
                     } else {
 #pragma unroll
                         for (int sp = QS - 1; sp >= 0; --sp) {
                             const uint4 b = q_op(sp, nb, j);
-                            mma16<C>(s[nb], kr[0][j].x, kr[1][j].x, kr[0][j].y, kr[1][j].y, b.x, b.y);
-                            mma16<C>(s[nb], kr[0][j].z, kr[1][j].z, kr[0][j].w, kr[1][j].w, b.z, b.w);
+                            mma16<C>(sp ? s2 : s[nb], kr[0][j].x, kr[1][j].x, kr[0][j].y, kr[1][j].y, b.x, b.y);
+                            mma16<C>(QS == 1 || sp ? s2 : s[nb], kr[0][j].z, kr[1][j].z, kr[0][j].w, kr[1][j].w, b.z, b.w);
                         }
                     }
                 }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[nb][e] += s2[e];
             }
             load_k(off);
             // ---- masks and the running maximum
@@ -441,7 +462,7 @@ __global__ void __launch_bounds__(kThreads) paged_decode_kernel(const __grid_con
             for (int r = warp; r < ROWS; r += kWarps) {
                 float mr = -INFINITY, lr = 0.0f, orow[8];
                 if (r < rows) {
-                    const int x1 = min(tb * kTile, p0 + r / gs + 1);
+                    const int x1 = min(tb * kTile, p0 + token_of(r) + 1);
                     row_pass<T, C>(A, row_q(r), it.seq, head, ta * kTile, x1, mr, lr, orow);
                     const float lift = exp2f(kLift);
                     lr *= lift;
@@ -514,38 +535,45 @@ __global__ void __launch_bounds__(kThreads) paged_decode_kernel(const __grid_con
             if (s_last) {  // uniform
                 __threadfence();
                 auto part_of = [&](int cta) { return P.parts + it.slot_of(cta) * ROWS * (D + 2); };
-                // every row's maximum over the parts (s_m[0]) and sum (s_l[0])
-                for (int r = warp; r < rows; r += kWarps) {
-                    float M = -INFINITY;
-                    for (int i = c0 + lane; i <= c1; i += 32) M = fmaxf(M, __ldcg(part_of(i) + ROWS * D + r));
-#pragma unroll
-                    for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
-                    const float base = M == -INFINITY ? 0.0f : M;
-                    float L = 0.0f;
-                    for (int i = c0 + lane; i <= c1; i += 32) {
-                        const float *pp = part_of(i) + ROWS * D;
-                        L = fmaf(ex2(__ldcg(pp + r) - base), __ldcg(pp + ROWS + r), L);
-                    }
-                    L = warp_sum(L);
-                    if (lane == 0) s_m[0][r] = base, s_l[0][r] = L;
-                }
-                __syncthreads();
                 constexpr int PER = ROWS * D / 4 / kThreads;  // float4 of the result per thread
                 float4 acc[PER];
 #pragma unroll
                 for (int k = 0; k < PER; ++k) acc[k] = make_float4(0, 0, 0, 0);
+                // 128 parts at a time: their maxima and sums to shared memory (thread = part), the
+                // running maximum and sum of every row (warp = row), the weights, the values
                 for (int b = c0; b <= c1; b += kThreads) {
                     const int cnt = min(kThreads, c1 + 1 - b);
-                    for (int i = tid; i < cnt * rows; i += kThreads) {
-                        const int r = i / cnt, w = i % cnt;
-                        s_w[r][w] = ex2(__ldcg(part_of(b + w) + ROWS * D + r) - s_m[0][r]);
+                    if (tid < cnt) {
+                        const float *pp = part_of(b + tid) + ROWS * D;
+                        for (int r = 0; r < rows; ++r) s_w[r][tid] = __ldcg(pp + r), s_p[r][tid] = __ldcg(pp + ROWS + r);
+                    }
+                    __syncthreads();
+                    for (int r = warp; r < rows; r += kWarps) {
+                        const float m0 = b == c0 ? -INFINITY : s_m[0][r], l0 = b == c0 ? 0.0f : s_l[0][r];
+                        float M = m0;
+                        for (int i = lane; i < cnt; i += 32) M = fmaxf(M, s_w[r][i]);
+#pragma unroll
+                        for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+                        const float base = M == -INFINITY ? 0.0f : M;
+                        float L = 0.0f;
+                        for (int i = lane; i < cnt; i += 32) {
+                            const float f = ex2(s_w[r][i] - base);
+                            s_w[r][i] = f;
+                            L = fmaf(f, s_p[r][i], L);
+                        }
+                        L = warp_sum(L);
+                        const float old = ex2(m0 - base);
+                        __syncwarp();
+                        if (lane == 0) s_m[0][r] = M, s_l[0][r] = fmaf(old, l0, L), s_c[r] = old;
                     }
                     __syncthreads();
 #pragma unroll
                     for (int k = 0; k < PER; ++k) {
                         const int i = tid + k * kThreads, r = i / (D / 4), d = (i % (D / 4)) * 4;
                         if (r < rows) {
-#pragma unroll 8
+                            const float old = s_c[r];
+                            acc[k].x *= old, acc[k].y *= old, acc[k].z *= old, acc[k].w *= old;
+#pragma unroll 16
                             for (int w = 0; w < cnt; ++w) {
                                 const float4 x = __ldcg(reinterpret_cast<const float4 *>(part_of(b + w) + r * D + d));
                                 const float f = s_w[r][w];
@@ -591,7 +619,7 @@ int launch_decode_t(const PagedAttnArgs &a, cudaStream_t st) {
     const int G = a.n_heads / a.n_kv_heads;
     P.sets = (G + 8 * NB - 1) / (8 * NB);
     P.g_set = (G + P.sets - 1) / P.sets;
-    P.line = {8 * NB / P.g_set, a.n_kv_heads * P.sets, 2, -1};
+    P.line = {8 * NB / P.g_set, a.n_kv_heads * P.sets, 2, 1, -1};
     // no more CTAs than there can be tiles
     const long long items = (long long)P.line.heads * (a.b.n_seqs + (long long)a.b.n_tokens / P.line.tq);
     const long long most = items * ((std::max(1, a.b.max_len) + kTile - 1) / kTile);
