@@ -4,6 +4,8 @@
 
 #include <cuda_bf16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "kernels.h"
 
@@ -27,6 +29,31 @@ template <>
 __device__ __forceinline__ __half el_from_f<__half>(float v) { return __float2half_rn(v); }
 template <>
 __device__ __forceinline__ __nv_bfloat16 el_from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// two fp32 in one register pair: one instruction for both
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    return v;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float &a, float &b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t v;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
 
 // N consecutive elements as one load or store of N * sizeof(T) <= 16 bytes (N = 8 fp32: two).
 template <typename T, int N>
@@ -67,6 +94,30 @@ struct ElVec {
             T t;
             memcpy(&t, &b, 2);
             return el_to_f<T>(t);
+        }
+    }
+    // elements 2 i and 2 i + 1
+    __device__ __forceinline__ uint64_t get2(int i) const {
+        if constexpr (sizeof(T) == 4) return pair(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+        else if constexpr (sizeof(T) == 2) {
+            if constexpr (std::is_same<T, __half>::value) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+                return pair(f.x, f.y);
+            } else {
+                return pair(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+            }
+        }
+    }
+    __device__ __forceinline__ void set2(int i, uint64_t v) {
+        float a, b;
+        unpair(v, a, b);
+        if constexpr (sizeof(T) == 4) w[2 * i] = __float_as_uint(a), w[2 * i + 1] = __float_as_uint(b);
+        else if constexpr (std::is_same<T, __half>::value) {
+            const __half2 h = __floats2half2_rn(a, b);
+            w[i] = *reinterpret_cast<const uint32_t *>(&h);
+        } else {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+            w[i] = *reinterpret_cast<const uint32_t *>(&h);
         }
     }
     __device__ __forceinline__ void set(const float *v) {

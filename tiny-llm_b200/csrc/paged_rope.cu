@@ -25,7 +25,8 @@ namespace tqb200 {
 namespace {
 
 constexpr int kRopeThreads = 128;
-constexpr int kRopeUnroll = 4;  // row groups whose loads are in flight together
+constexpr int kRopeUnroll = 2;  // row groups per step; the next step's loads are in flight
+constexpr int kRopePerSm = 5;   // CTAs per SM
 
 struct RopeParams {
     RopeArgs a;
@@ -33,46 +34,51 @@ struct RopeParams {
     BatchView b;
     int *status;
     int lane_bits;           // log2 of the lanes of a row
-    int warps;               // warps per token
+    int warps;               // parts that a token is cut into, a warp each
     double log2_step;        // log2(theta) / h: frequency i is 2^(-i log2_step)
     double ratio;            // 2^-log2_step
 };
 
-// The row's place in its sequence; false: the row is left as it is.
-template <bool APPEND>
-__device__ __forceinline__ bool row_place(const RopeParams &P, int tok, int *table_row, int *cache_pos,
-                                          int *rope_pos) {
-    *cache_pos = 0;
-    *table_row = 0;
-    if constexpr (APPEND) {
-        const int s = seq_of_row(P.b, tok);
-        const SeqInfo q = seq_info(P.b, s);
-        if (!q.ok) {
-            if ((threadIdx.x & 31) == 0) report(P.status, TQB200_PAGED_BAD_SEQ);
-            return false;
+// The token's place in its sequence; live == false: its rows are left as they are.  A sequence
+// once found serves the following tokens without a search.
+struct Place {
+    SeqInfo q{0, 0, 0, 0};
+    int seq = 0, cache_pos = 0, rope_pos = 0;
+    bool live = false;
+    template <bool APPEND>
+    __device__ __forceinline__ void find(const RopeParams &P, int tok) {
+        live = true;
+        cache_pos = 0;
+        if constexpr (APPEND) {
+            if (!q.ok || tok < q.q0 || tok >= q.q0 + q.n) {
+                seq = seq_of_row(P.b, tok);
+                q = seq_info(P.b, seq);
+                if (!q.ok && (threadIdx.x & 31) == 0) report(P.status, TQB200_PAGED_BAD_SEQ);
+                live = q.ok && tok >= q.q0 && tok < q.q0 + q.n;
+            }
+            cache_pos = q.len - q.n + (tok - q.q0);
         }
-        if (tok < q.q0 || tok >= q.q0 + q.n) return false;
-        *table_row = s;
-        *cache_pos = q.len - q.n + (tok - q.q0);
+        rope_pos = P.a.positions && live ? P.a.positions[tok] : cache_pos;
     }
-    *rope_pos = P.a.positions ? P.a.positions[tok] : *cache_pos;
-    return true;
-}
+};
 
-template <typename T, typename C, bool APPEND>
-__global__ void __launch_bounds__(kRopeThreads) rope_vec_kernel(const __grid_constant__ RopeParams P) {
-    constexpr int VEC = 16 / sizeof(T);
+// LB: log2 of the lanes of a row, -1 where it is known at run time only.
+template <typename T, typename C, bool APPEND, int LB>
+__global__ void __launch_bounds__(kRopeThreads, kRopePerSm) rope_vec_kernel(const __grid_constant__ RopeParams P) {
+    constexpr int VEC = 16 / sizeof(T), H = VEC / 2;
+    constexpr int U = kRopeUnroll;
     const RopeArgs &a = P.a;
     const long long gw = (long long)blockIdx.x * (kRopeThreads / 32) + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
-    const long long tok_ll = gw / P.warps;
-    if (tok_ll >= a.n_tokens) return;  // warp-uniform; no CTA barrier below
-    const int tok = (int)tok_ll, part = (int)(gw - tok_ll * P.warps);
-    int seq, pos, rpos;
-    if (!row_place<APPEND>(P, tok, &seq, &pos, &rpos)) return;
+    // warp gw: part `part` of tokens tok, tok + step, ... (step: whole tokens at a time)
+    const int part = (int)(gw % P.warps);
+    const long long step = (long long)gridDim.x * (kRopeThreads / 32) / P.warps;
+    long long tok = gw / P.warps;
+    if (tok >= step || tok >= a.n_tokens) return;  // warp-uniform; no CTA barrier below
 
-    const int lpr = 1 << P.lane_bits, rpi = 32 >> P.lane_bits;
-    const int sub = lane >> P.lane_bits, c = lane & (lpr - 1);
+    const int bits = LB >= 0 ? LB : P.lane_bits;
+    const int lpr = 1 << bits, rpi = 32 >> bits;
+    const int sub = lane >> bits, c = lane & (lpr - 1);
     const bool in_row = c * VEC < a.head_dim;
     const int hc = a.rotary_dim / 2 / VEC;  // lanes of one rotated half
     const bool rot = c < 2 * hc, low = c < hc;
@@ -80,137 +86,178 @@ __global__ void __launch_bounds__(kRopeThreads) rope_vec_kernel(const __grid_con
     // row groups: n_q of queries, n_k of keys, then (append) n_k of values
     const int n_q = (a.n_heads + rpi - 1) / rpi, n_k = (a.n_kv_heads + rpi - 1) / rpi;
     const int n_it = n_q + (APPEND ? 2 : 1) * n_k;
+    const int mine = sub * a.head_dim + c * VEC;  // the lane's elements in a group of rows
+    const int apart = rpi * a.head_dim;           // from one group to the next
 
-    auto source = [&](int it, int &head, int &count) -> const T * {
-        const char *base;
-        long long stride;
-        if (it < n_q) base = (const char *)a.q, stride = a.q_stride, count = a.n_heads;
-        else if (it < n_q + n_k) it -= n_q, base = (const char *)a.k, stride = a.k_stride, count = a.n_kv_heads;
-        else it -= n_q + n_k, base = (const char *)a.v, stride = a.v_stride, count = a.n_kv_heads;
-        head = it * rpi + sub;
-        return reinterpret_cast<const T *>(base) + tok * stride + (long long)head * a.head_dim + c * VEC;
-    };
-    ElVec<T, VEC> raw[kRopeUnroll];
-    auto load_group = [&](int it0) {
+    auto load_group = [&](ElVec<T, VEC> (&raw)[U], long long t, int it0) {
+        const bool any = t < a.n_tokens;
+        const T *q = (const T *)a.q + t * a.q_stride + mine;
+        const T *k = (const T *)a.k + t * a.k_stride + mine - (long long)n_q * apart;
+        const T *v = (const T *)a.v + t * a.v_stride + mine - (long long)(n_q + n_k) * apart;
 #pragma unroll
-        for (int u = 0; u < kRopeUnroll; ++u) {
+        for (int u = 0; u < U; ++u) {
             const int it = it0 + u * P.warps;
 #pragma unroll
             for (int w = 0; w < 4; ++w) raw[u].w[w] = 0u;
-            if (it < n_it) {
-                int head, count;
-                const T *p = source(it, head, count);
-                if (head < count && in_row) raw[u].load(p);
-            }
+            // rows behind the last head: the group's lanes there have nothing
+            const int head = (it < n_q ? it : it < n_q + n_k ? it - n_q : it - n_q - n_k) * rpi + sub;
+            const T *p = it < n_q ? q : APPEND && it >= n_q + n_k ? v : k;
+            if (any && it < n_it && in_row && head < (it < n_q ? a.n_heads : a.n_kv_heads)) raw[u].load(p + (long long)it * apart);
         }
     };
-    load_group(part);
+    ElVec<T, VEC> raw[U];
+    load_group(raw, tok, part);
 
-    // where this token's keys and values go, and its angles
-    long long slot = -1;
-    if constexpr (APPEND) {
-        if (pos >= 0 && a.n_kv_heads > 0) {
-            int bad = 0;
-            slot = P.kv.offset(P.b.table + (long long)seq * P.b.table_stride, pos, 0, &bad);
-            if (bad && lane == 0) report(P.status, TQB200_PAGED_BAD_PAGE);
-        }
-    }
-    float fq[2][VEC], fk[2][VEC];  // factors of x and of its partner
+    // The lanes of one pair index (two halves of rpi rows) share its VEC angles: lane (sub, half)
+    // forms `share` of them, from number slot * share on; their frequencies stay over the tokens.
+    const int pc = c + (rot ? (low ? hc : -hc) : 0);  // the partner's lane in the row
+    const int share = VEC / min(VEC, 2 * rpi);        // angles per lane
+    const int slot = share > 2 ? 0 : (sub * 2 + (low ? 0 : 1)) % (VEC / share);
+    double freq[2];                                   // turns per position
     {
-        float cs[VEC], sn[VEC];
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) cs[j] = 1.0f, sn[j] = 0.0f;
-        if (rot) {
-            const int i0 = (low ? c : c - hc) * VEC;
-            double f = exp2(-(double)i0 * P.log2_step) * 0.15915494309189533577;  // turns per position
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                double t = (double)rpos * f;
-                t -= rint(t);
-                float s_, c_;
-                sincospif(2.0f * (float)t, &s_, &c_);
-                cs[j] = c_;
-                sn[j] = low ? -s_ : s_;
-                f *= P.ratio;
-            }
-        }
-        const int pc = c + (rot ? (low ? hc : -hc) : 0);  // the partner's lane in the row
-        auto factors = [&](const float *w, float (&f)[2][VEC]) {
-            if (w == nullptr || !in_row) {
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) f[0][j] = cs[j], f[1][j] = sn[j];
-            } else {
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    f[0][j] = w[c * VEC + j] * cs[j];
-                    f[1][j] = w[pc * VEC + j] * sn[j];
-                }
-            }
-        };
-        factors(a.q_norm, fq);
-        factors(a.k_norm, fk);
+        const double i0 = (low ? c : c - hc) * VEC + slot * share;
+        freq[0] = rot ? exp2(-i0 * P.log2_step) * 0.15915494309189533577 : 0.0;
+        freq[1] = freq[0] * P.ratio;
     }
 
     const float inv_n = 1.0f / (float)a.head_dim;
-    auto turn = [&](const ElVec<T, VEC> &x, const float (&f)[2][VEC], bool norm, float (&y)[VEC]) {
-        float r = 1.0f;
-        if (norm) {
-            float ss = 0.0f;
+    auto turn = [&](const ElVec<T, VEC> &x, const uint64_t (&f)[2][H], bool norm, uint64_t (&y)[H]) {
+        uint64_t r = pair(1.0f, 1.0f);
+        uint64_t x2[H];
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) ss = fmaf(x.get(j), x.get(j), ss);
+        for (int j = 0; j < H; ++j) x2[j] = x.get2(j);
+        if (norm) {
+            uint64_t ss2 = mul2(x2[0], x2[0]);
+#pragma unroll
+            for (int j = 1; j < H; ++j) ss2 = fma2(x2[j], x2[j], ss2);
+            float ss, sb;
+            unpair(ss2, ss, sb);
+            ss += sb;
+#pragma unroll
             for (int o = lpr >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            r = rsqrtf(fmaf(ss, inv_n, a.eps));
+            ss = rsqrtf(fmaf(ss, inv_n, a.eps));
+            r = pair(ss, ss);
         }
         ElVec<T, VEC> xp;
+        // lanes without a rotation take no partner: 0 * its infinity would be NaN
 #pragma unroll
-        for (int w = 0; w < 4; ++w) xp.w[w] = __shfl_sync(0xffffffffu, x.w[w], partner);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            // lanes without a rotation keep x alone: 0 * a partner's infinity would be NaN
-            const float other = rot ? xp.get(j) * f[1][j] : 0.0f;
-            y[j] = r * fmaf(x.get(j), f[0][j], other);
+        for (int w = 0; w < 4; ++w) {
+            xp.w[w] = __shfl_sync(0xffffffffu, x.w[w], partner);
+            if (!rot) xp.w[w] = 0u;
         }
+#pragma unroll
+        for (int j = 0; j < H; ++j) y[j] = mul2(r, fma2(xp.get2(j), f[1][j], mul2(x2[j], f[0][j])));
     };
 
-    for (int it0 = part; it0 < n_it; it0 += kRopeUnroll * P.warps) {
-        if (it0 != part) load_group(it0);
+    Place place;
+    for (; tok < a.n_tokens; tok += step) {
+        place.find<APPEND>(P, (int)tok);
+        // where this token's keys and values go
+        long long at = -1;
+        if constexpr (APPEND) {
+            if (place.live && place.cache_pos >= 0) {
+                int bad = 0;
+                at = P.kv.offset(P.b.table + (long long)place.seq * P.b.table_stride, place.cache_pos, 0, &bad);
+                if (bad && lane == 0) report(P.status, TQB200_PAGED_BAD_PAGE);
+            }
+        }
+        // its angles, and the factors of x and of the partner's x
+        uint64_t fq[2][H], fk[2][H];
+        {
+            float cv[2], sv[2];
 #pragma unroll
-        for (int u = 0; u < kRopeUnroll; ++u) {
-            const int it = it0 + u * P.warps;
-            if (it >= n_it) break;  // warp-uniform
-            float y[VEC];
-            if (it < n_q) {
-                turn(raw[u], fq, a.q_norm != nullptr, y);
-                const int head = it * rpi + sub;
-                if (head < a.n_heads && in_row) {
-                    ElVec<T, VEC> o;
-                    o.set(y);
-                    o.store((T *)a.q_out + tok * a.q_out_stride + (long long)head * a.head_dim + c * VEC);
-                }
-            } else if (it < n_q + n_k) {
-                turn(raw[u], fk, a.k_norm != nullptr, y);
-                const int head = (it - n_q) * rpi + sub;
-                if (head < a.n_kv_heads && in_row) {
-                    if constexpr (APPEND) {
-                        ElVec<C, VEC> o;
-                        o.set(y);
-                        if (slot >= 0) o.store((C *)P.kv.k + slot + head * P.kv.head_stride + c * VEC);
-                    } else {
-                        ElVec<T, VEC> o;
-                        o.set(y);
-                        o.store((T *)a.k_out + tok * a.k_out_stride + (long long)head * a.head_dim + c * VEC);
+            for (int e = 0; e < 2; ++e) {
+                double t = (double)place.rope_pos * freq[e];
+                t -= rint(t);
+                sincospif(2.0f * (float)t, &sv[e], &cv[e]);
+            }
+            float cs[VEC], sn[VEC];
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                // angle j of this lane's pair indexes: formed by the lane of slot j / share among
+                // those that share them
+                if (share > 2) {
+                    // few lanes share (wide rows): each forms its own, one by one
+                    double f = freq[0];
+                    for (int k = 0; k < j; ++k) f *= P.ratio;
+                    double t = (double)place.rope_pos * f;
+                    t -= rint(t);
+                    sincospif(2.0f * (float)t, &sn[j], &cs[j]);
+                } else {
+                    const int from = j / share, s_ = from >> 1, h_ = from & 1;
+                    const int src = rot ? (s_ << bits) + (low ? c : c - hc) + (h_ ? hc : 0) : lane;
+                    cs[j] = __shfl_sync(0xffffffffu, cv[0], src);
+                    sn[j] = __shfl_sync(0xffffffffu, sv[0], src);
+                    if (share == 2) {
+                        const float c1 = __shfl_sync(0xffffffffu, cv[1], src), s1 = __shfl_sync(0xffffffffu, sv[1], src);
+                        if (j & 1) cs[j] = c1, sn[j] = s1;
                     }
                 }
-            } else if constexpr (APPEND) {
-                const int head = (it - n_q - n_k) * rpi + sub;
-                if (head < a.n_kv_heads && in_row && slot >= 0) {
+                if (!rot) cs[j] = 1.0f, sn[j] = 0.0f;
+                else if (low) sn[j] = -sn[j];
+            }
+            auto factors = [&](const float *w, uint64_t (&f)[2][H]) {
+                const bool has = w && in_row;
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) y[j] = raw[u].get(j);
-                    ElVec<C, VEC> o;
-                    o.set(y);
-                    o.store((C *)P.kv.v + slot + head * P.kv.head_stride + c * VEC);
+                for (int j = 0; j < H; ++j) {
+                    const float2 own = has ? *reinterpret_cast<const float2 *>(w + c * VEC + 2 * j) : make_float2(1.0f, 1.0f);
+                    const float2 his = has ? *reinterpret_cast<const float2 *>(w + pc * VEC + 2 * j) : make_float2(1.0f, 1.0f);
+                    f[0][j] = pair(own.x * cs[2 * j], own.y * cs[2 * j + 1]);
+                    f[1][j] = pair(his.x * sn[2 * j], his.y * sn[2 * j + 1]);
+                }
+            };
+            factors(a.q_norm, fq);
+            factors(a.k_norm, fk);
+        }
+        T *q_to = (T *)a.q_out + tok * a.q_out_stride + mine;
+        T *k_to = (T *)a.k_out + tok * a.k_out_stride + mine - (long long)n_q * apart;
+        const long long cache_to = at + sub * P.kv.head_stride + c * VEC, cache_apart = rpi * P.kv.head_stride;
+        for (int it0 = part; it0 < n_it; it0 += U * P.warps) {
+            // the next row groups (or the next token's first) are in flight while these are used
+            ElVec<T, VEC> ahead[U];
+            const bool more = it0 + U * P.warps < n_it;
+            load_group(ahead, more ? tok : tok + step, more ? it0 + U * P.warps : part);
+            if (place.live) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int it = it0 + u * P.warps;
+                    if (it >= n_it) break;  // warp-uniform
+                    uint64_t y[H];
+                    if (it < n_q) {
+                        turn(raw[u], fq, a.q_norm != nullptr, y);
+                        if (it * rpi + sub < a.n_heads && in_row) {
+                            ElVec<T, VEC> o;
+#pragma unroll
+                            for (int j = 0; j < H; ++j) o.set2(j, y[j]);
+                            o.store(q_to + (long long)it * apart);
+                        }
+                    } else if (it < n_q + n_k) {
+                        turn(raw[u], fk, a.k_norm != nullptr, y);
+                        if ((it - n_q) * rpi + sub < a.n_kv_heads && in_row) {
+                            if constexpr (APPEND) {
+                                ElVec<C, VEC> o;
+#pragma unroll
+                                for (int j = 0; j < H; ++j) o.set2(j, y[j]);
+                                if (at >= 0) o.store((C *)P.kv.k + cache_to + (it - n_q) * cache_apart);
+                            } else {
+                                ElVec<T, VEC> o;
+#pragma unroll
+                                for (int j = 0; j < H; ++j) o.set2(j, y[j]);
+                                o.store(k_to + (long long)it * apart);
+                            }
+                        }
+                    } else if constexpr (APPEND) {
+                        if ((it - n_q - n_k) * rpi + sub < a.n_kv_heads && in_row && at >= 0) {
+                            ElVec<C, VEC> o;
+#pragma unroll
+                            for (int j = 0; j < H; ++j) o.set2(j, raw[u].get2(j));
+                            o.store((C *)P.kv.v + cache_to + (it - n_q - n_k) * cache_apart);
+                        }
+                    }
                 }
             }
+#pragma unroll
+            for (int u = 0; u < U; ++u) raw[u] = ahead[u];
         }
     }
 }
@@ -226,8 +273,10 @@ __global__ void __launch_bounds__(kRopeThreads) rope_any_kernel(const __grid_con
     const long long tok_ll = gw / rows;
     if (tok_ll >= a.n_tokens) return;
     const int tok = (int)tok_ll, row = (int)(gw - tok_ll * rows);
-    int seq, pos, rpos;
-    if (!row_place<APPEND>(P, tok, &seq, &pos, &rpos)) return;
+    Place place;
+    place.find<APPEND>(P, tok);
+    if (!place.live) return;
+    const int pos = place.cache_pos, rpos = place.rope_pos, seq = place.seq;
     const int D = a.head_dim, half = a.rotary_dim / 2;
     const bool is_q = row < a.n_heads, is_v = row >= a.n_heads + a.n_kv_heads;
     const int head = is_q ? row : is_v ? row - a.n_heads - a.n_kv_heads : row - a.n_heads;
@@ -297,6 +346,7 @@ int launch_rope_t(RopeParams &P, cudaStream_t st) {
     while (lanes * VEC < a.head_dim) lanes *= 2, ++bits;
     bool vec = lanes <= 32 && a.head_dim % VEC == 0 && (a.rotary_dim / 2) % VEC == 0;
     vec = vec && multiple((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.q_out | (uintptr_t)a.k_out, 16);
+    vec = vec && multiple((uintptr_t)a.q_norm | (uintptr_t)a.k_norm, 8);
     vec = vec && multiple((uintptr_t)(a.q_stride | a.k_stride | a.v_stride | a.q_out_stride | a.k_out_stride), VEC);
     if (APPEND)
         vec = vec && multiple((uintptr_t)P.kv.k | (uintptr_t)P.kv.v, 16) &&
@@ -306,14 +356,25 @@ int launch_rope_t(RopeParams &P, cudaStream_t st) {
         P.lane_bits = bits;
         const int rpi = 32 >> bits;
         const int n_it = (a.n_heads + rpi - 1) / rpi + (APPEND ? 2 : 1) * ((a.n_kv_heads + rpi - 1) / rpi);
-        // warps per token: enough for 16 warps per SM, each with as many row groups as the others
-        const int target = 16 * num_sms();
-        int warps = std::min(n_it, (target + a.n_tokens - 1) / a.n_tokens);
-        const int per = (n_it + warps - 1) / warps;
-        P.warps = (n_it + per - 1) / per;
-        const long long blocks = ((long long)a.n_tokens * P.warps + kWarps - 1) / kWarps;
-        TQ_CHECK_ARG(blocks < (1LL << 31), "norm/rope: %d tokens", a.n_tokens);
-        rope_vec_kernel<T, C, APPEND><<<(unsigned)blocks, kRopeThreads, 0, st>>>(P);
+        // The resident warps stay and take further tokens.  A token is cut into `parts` (its row
+        // groups dealt out) so that few tokens still reach every warp, and so that the last
+        // round is full: the cost of parts p is the rounds times a part's groups and its
+        // set-up, worth about 3 of them.
+        const long long resident = (long long)kRopePerSm * num_sms() * kWarps;
+        int parts = 1;
+        double best = 0.0;
+        for (int p = 1; p <= std::min(n_it, 64); ++p) {
+            const double rounds = std::ceil((double)a.n_tokens * p / (double)(resident / p * p));
+            const double cost = rounds * ((n_it + p - 1) / p + 3);
+            if (p == 1 || cost < best) best = cost, parts = p;
+            if (p >= 4 && (long long)a.n_tokens * p >= resident) break;
+        }
+        P.warps = parts;
+        const long long blocks = std::min(((long long)a.n_tokens * parts + kWarps - 1) / kWarps, resident / kWarps);
+        if (bits == 3) rope_vec_kernel<T, C, APPEND, 3><<<(unsigned)blocks, kRopeThreads, 0, st>>>(P);
+        else if (bits == 4) rope_vec_kernel<T, C, APPEND, 4><<<(unsigned)blocks, kRopeThreads, 0, st>>>(P);
+        else if (bits == 5) rope_vec_kernel<T, C, APPEND, 5><<<(unsigned)blocks, kRopeThreads, 0, st>>>(P);
+        else rope_vec_kernel<T, C, APPEND, -1><<<(unsigned)blocks, kRopeThreads, 0, st>>>(P);
     } else {
         const int rows = a.n_heads + (APPEND ? 2 : 1) * a.n_kv_heads;
         const long long blocks = ((long long)a.n_tokens * rows + kWarps - 1) / kWarps;
