@@ -25,7 +25,7 @@ namespace tqb200 {
 namespace {
 
 constexpr int kRopeThreads = 128;
-constexpr int kRopeUnroll = 2;  // row groups per step; the next step's loads are in flight
+constexpr int kRopeUnroll = 4;  // row groups whose loads are in flight together
 constexpr int kRopePerSm = 5;   // CTAs per SM
 
 struct RopeParams {
@@ -83,30 +83,20 @@ __global__ void __launch_bounds__(kRopeThreads, kRopePerSm) rope_vec_kernel(cons
     const int hc = a.rotary_dim / 2 / VEC;  // lanes of one rotated half
     const bool rot = c < 2 * hc, low = c < hc;
     const int partner = lane + (rot ? (low ? hc : -hc) : 0);
-    // row groups: n_q of queries, n_k of keys, then (append) n_k of values
+    // Row groups: n_q of queries, n_k of keys, then (append) n_k of values; group i of them all
+    // belongs to part i % warps.  first_*: this part's first of each kind; lim_*: how many
+    // groups hold a row for this lane.
     const int n_q = (a.n_heads + rpi - 1) / rpi, n_k = (a.n_kv_heads + rpi - 1) / rpi;
-    const int n_it = n_q + (APPEND ? 2 : 1) * n_k;
-    const int mine = sub * a.head_dim + c * VEC;  // the lane's elements in a group of rows
-    const int apart = rpi * a.head_dim;           // from one group to the next
-
-    auto load_group = [&](ElVec<T, VEC> (&raw)[U], long long t, int it0) {
-        const bool any = t < a.n_tokens;
-        const T *q = (const T *)a.q + t * a.q_stride + mine;
-        const T *k = (const T *)a.k + t * a.k_stride + mine - (long long)n_q * apart;
-        const T *v = (const T *)a.v + t * a.v_stride + mine - (long long)(n_q + n_k) * apart;
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int it = it0 + u * P.warps;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) raw[u].w[w] = 0u;
-            // rows behind the last head: the group's lanes there have nothing
-            const int head = (it < n_q ? it : it < n_q + n_k ? it - n_q : it - n_q - n_k) * rpi + sub;
-            const T *p = it < n_q ? q : APPEND && it >= n_q + n_k ? v : k;
-            if (any && it < n_it && in_row && head < (it < n_q ? a.n_heads : a.n_kv_heads)) raw[u].load(p + (long long)it * apart);
-        }
-    };
-    ElVec<T, VEC> raw[U];
-    load_group(raw, tok, part);
+    const int first_q = part, first_k = (part + P.warps - n_q % P.warps) % P.warps;
+    const int first_v = (part + P.warps - (n_q + n_k) % P.warps) % P.warps;
+    const int lim_q = in_row ? (a.n_heads - sub + rpi - 1) / rpi : 0, lim_k = in_row ? (a.n_kv_heads - sub + rpi - 1) / rpi : 0;
+    const int mine = sub * a.head_dim + c * VEC;        // the lane's elements in a group of rows
+    const long long apart = (long long)P.warps * rpi * a.head_dim;  // from one of this part's groups to the next
+    const T *const q0 = (const T *)a.q + mine + (long long)first_q * rpi * a.head_dim;
+    const T *const k0 = (const T *)a.k + mine + (long long)first_k * rpi * a.head_dim;
+    const T *const v0 = (const T *)a.v + mine + (long long)first_v * rpi * a.head_dim;
+    T *const qo0 = (T *)a.q_out + mine + (long long)first_q * rpi * a.head_dim;
+    T *const ko0 = (T *)a.k_out + mine + (long long)first_k * rpi * a.head_dim;
 
     // The lanes of one pair index (two halves of rpi rows) share its VEC angles: lane (sub, half)
     // forms `share` of them, from number slot * share on; their frequencies stay over the tokens.
@@ -209,55 +199,76 @@ __global__ void __launch_bounds__(kRopeThreads, kRopePerSm) rope_vec_kernel(cons
             factors(a.q_norm, fq);
             factors(a.k_norm, fk);
         }
-        T *q_to = (T *)a.q_out + tok * a.q_out_stride + mine;
-        T *k_to = (T *)a.k_out + tok * a.k_out_stride + mine - (long long)n_q * apart;
-        const long long cache_to = at + sub * P.kv.head_stride + c * VEC, cache_apart = rpi * P.kv.head_stride;
-        for (int it0 = part; it0 < n_it; it0 += U * P.warps) {
-            // the next row groups (or the next token's first) are in flight while these are used
-            ElVec<T, VEC> ahead[U];
-            const bool more = it0 + U * P.warps < n_it;
-            load_group(ahead, more ? tok : tok + step, more ? it0 + U * P.warps : part);
-            if (place.live) {
+        // One kind of rows: U groups' loads at a time, then what is done with each.
+        auto rows = [&](const T *src, int it, int groups, int lim, auto &&use) {
+            for (; it < groups; it += U * P.warps) {
+                ElVec<T, VEC> raw[U];
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    const int it = it0 + u * P.warps;
-                    if (it >= n_it) break;  // warp-uniform
-                    uint64_t y[H];
-                    if (it < n_q) {
-                        turn(raw[u], fq, a.q_norm != nullptr, y);
-                        if (it * rpi + sub < a.n_heads && in_row) {
-                            ElVec<T, VEC> o;
 #pragma unroll
-                            for (int j = 0; j < H; ++j) o.set2(j, y[j]);
-                            o.store(q_to + (long long)it * apart);
-                        }
-                    } else if (it < n_q + n_k) {
-                        turn(raw[u], fk, a.k_norm != nullptr, y);
-                        if ((it - n_q) * rpi + sub < a.n_kv_heads && in_row) {
-                            if constexpr (APPEND) {
-                                ElVec<C, VEC> o;
+                    for (int w = 0; w < 4; ++w) raw[u].w[w] = 0u;
+                    if (it + u * P.warps < lim) raw[u].load(src);
+                    src += apart;
+                }
 #pragma unroll
-                                for (int j = 0; j < H; ++j) o.set2(j, y[j]);
-                                if (at >= 0) o.store((C *)P.kv.k + cache_to + (it - n_q) * cache_apart);
-                            } else {
-                                ElVec<T, VEC> o;
-#pragma unroll
-                                for (int j = 0; j < H; ++j) o.set2(j, y[j]);
-                                o.store(k_to + (long long)it * apart);
-                            }
-                        }
-                    } else if constexpr (APPEND) {
-                        if ((it - n_q - n_k) * rpi + sub < a.n_kv_heads && in_row && at >= 0) {
-                            ElVec<C, VEC> o;
-#pragma unroll
-                            for (int j = 0; j < H; ++j) o.set2(j, raw[u].get2(j));
-                            o.store((C *)P.kv.v + cache_to + (it - n_q - n_k) * cache_apart);
-                        }
-                    }
+                for (int u = 0; u < U; ++u) {
+                    if (it + u * P.warps >= groups) break;  // warp-uniform
+                    use(raw[u], it + u * P.warps < lim);
                 }
             }
+        };
+        if (!place.live) continue;
+        {
+            T *to = qo0 + tok * a.q_out_stride;
+            rows(q0 + tok * a.q_stride, first_q, n_q, lim_q, [&](const ElVec<T, VEC> &x, bool has) {
+                uint64_t y[H];
+                turn(x, fq, a.q_norm != nullptr, y);
+                if (has) {
+                    ElVec<T, VEC> o;
 #pragma unroll
-            for (int u = 0; u < U; ++u) raw[u] = ahead[u];
+                    for (int j = 0; j < H; ++j) o.set2(j, y[j]);
+                    o.store(to);
+                }
+                to += apart;
+            });
+        }
+        if constexpr (!APPEND) {
+            T *to = ko0 + tok * a.k_out_stride;
+            rows(k0 + tok * a.k_stride, first_k, n_k, lim_k, [&](const ElVec<T, VEC> &x, bool has) {
+                uint64_t y[H];
+                turn(x, fk, a.k_norm != nullptr, y);
+                if (has) {
+                    ElVec<T, VEC> o;
+#pragma unroll
+                    for (int j = 0; j < H; ++j) o.set2(j, y[j]);
+                    o.store(to);
+                }
+                to += apart;
+            });
+        } else if (at >= 0) {
+            const long long heads_apart = (long long)P.warps * rpi * P.kv.head_stride;
+            C *to = (C *)P.kv.k + at + (first_k * rpi + sub) * P.kv.head_stride + c * VEC;
+            rows(k0 + tok * a.k_stride, first_k, n_k, lim_k, [&](const ElVec<T, VEC> &x, bool has) {
+                uint64_t y[H];
+                turn(x, fk, a.k_norm != nullptr, y);
+                if (has) {
+                    ElVec<C, VEC> o;
+#pragma unroll
+                    for (int j = 0; j < H; ++j) o.set2(j, y[j]);
+                    o.store(to);
+                }
+                to += heads_apart;
+            });
+            to = (C *)P.kv.v + at + (first_v * rpi + sub) * P.kv.head_stride + c * VEC;
+            rows(v0 + tok * a.v_stride, first_v, n_k, lim_k, [&](const ElVec<T, VEC> &x, bool has) {
+                if (has) {
+                    ElVec<C, VEC> o;
+#pragma unroll
+                    for (int j = 0; j < H; ++j) o.set2(j, x.get2(j));
+                    o.store(to);
+                }
+                to += heads_apart;
+            });
         }
     }
 }
