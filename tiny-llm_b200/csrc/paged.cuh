@@ -594,6 +594,9 @@ struct Line {
     }
 };
 
+// A driver function by name, looked up at run time (the library links no driver API); null
+// where there is none.
+void *driver_entry(const char *name);
 int launch_qk_norm_rope(const RopeArgs &a, cudaStream_t st);
 int launch_paged_append(const RopeArgs &a, const PagedView &kv, int cache_type, const BatchView &b,
                         int *status, cudaStream_t st);

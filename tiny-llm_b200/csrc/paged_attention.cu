@@ -50,6 +50,17 @@ int launch_any(const PagedAttnArgs &a, cudaStream_t st) {
 
 }  // namespace
 
+void *driver_entry(const char *name) {
+    void *fn = nullptr;
+    cudaDriverEntryPointQueryResult q{};
+    if (cudaGetDriverEntryPointByVersion(name, &fn, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess) {
+        cudaGetLastError();
+        return nullptr;
+    }
+    return fn;
+}
+
 size_t paged_attention_work_bytes(int n_heads, int n_kv_heads, int head_dim) {
     (void)n_heads, (void)n_kv_heads;
     return head_dim == 64 || head_dim == 128

@@ -12,13 +12,12 @@
 // while one is in its softmax the other's products run.
 // Roles (warps): QT groups of 4 softmax warps (thread = query row = TMEM lane), 2 QT warps that
 // fetch keys and values, QT warps that each issue one query tile's products.
-//  * Keys and values come by 16-byte cp.async, one page lookup per position, so any page size
-//    and any layout of 16-byte aligned rows is read alike; a ring of slots holds whole K or V
-//    tiles in the order K0 V0 K1 V1 ...  A warp's 32 copies are 4 chunks of 8 positions, whose
-//    16-byte pieces are adjacent in shared memory (no bank conflicts).  Positions past the end
-//    and on bad pages are filled with zeros and marked in a bitmap.
-//  * Shared memory holds the canonical layout without swizzle: 8 x 16-byte core matrices, the
-//    D / 8 of 8 positions adjacent.  It serves K as the K-major and V as the MN-major B operand.
+//  * A ring of slots holds whole K or V tiles in the order they are used, K0 K1 V0 K2 V1 ...
+//    Whole tiles come by TMA from the pages (any order of heads and slots: the tensor map has
+//    the cache's strides), the others (a sequence's last, odd page sizes) by 16-byte cp.async
+//    with positions that do not exist filled with zeros; a bitmap per tile marks those.
+//  * Shared memory holds rows of 128 bytes (64 dimensions of a position or query row) in the
+//    128-byte swizzle, as K-major A and B operands for Q K^T and MN-major B operand for P V.
 //  * Softmax: the row's maximum is raised only when a score passes it by 2^8 (then the warp
 //    rescales its rows of O in TMEM); weights carry a factor 2^6 against fp16's subnormals,
 //    so they stay below 2^14.
@@ -26,6 +25,9 @@
 //    split into fp16 hi + lo, two products each: 22 bits of either operand.
 //  * Every wait is bounded; after one runs out the roles go on without waiting or issuing, the
 //    issued copies and products are waited for (bounded), TMEM is freed and the error stored.
+#include <cuda.h>
+#include <string.h>
+
 #include <algorithm>
 #include <type_traits>
 
@@ -40,7 +42,7 @@ constexpr int kBehind = 3;        // tiles whose copies a fetching warp leaves i
 constexpr int kRows = 128;        // query rows per tile: TMEM lanes
 constexpr int kMaxSlots = 12;
 constexpr int kMarks = 16;        // tiles whose bitmaps are kept (more than the ring holds)
-constexpr int KT = 64;            // positions per tile
+constexpr int KT = 64;            // positions per tile (two words of a bitmap)
 constexpr int kMeta = 1024;
 
 struct ChunkParams {
@@ -50,12 +52,17 @@ struct ChunkParams {
     LineShape line;
     int sets, g_set;
     int slots;
+    int box_rows;               // slots of a page per tensor copy, 0: no tensor copies
+    alignas(64) uint8_t map_k[128], map_v[128];
 };
 
 // ---------------------------------------------------------------- tcgen05
-__device__ __forceinline__ uint64_t core_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
-    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(sbo >> 4) << 32) |
-           (1ull << 46);
+// Operand in rows of 128 bytes (64 elements), 16-byte piece p of row r at p ^ (r & 7): swizzle
+// mode 2.  Eight rows are 1024 bytes (the stride offset); `lead` is the way from 64 elements to
+// the next 64 along the contiguous dimension of an MN-major operand.
+__device__ __forceinline__ uint64_t row_desc(uint32_t saddr, uint32_t lead) {
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           (1ull << 46) | (2ull << 61);
 }
 // kind::f16, fp32 accumulator, M = 128; bv: the B operand is MN-major
 template <typename C>
@@ -151,6 +158,12 @@ __device__ __forceinline__ bool test_once(uint64_t *bar, uint32_t parity) {
 __device__ __forceinline__ void copy16(uint32_t dst, const char *src, bool live) {  // not live: zeros
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void box_load(uint32_t dst, const void *map, int x, int y, int z, int w, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+        : "memory");
+}
 template <int N>
 __device__ __forceinline__ void copies_left() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
@@ -195,7 +208,7 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, ChunkShape<T, D
     paged_chunk_kernel(const __grid_constant__ ChunkParams P) {
     using Sh = ChunkShape<T, D, QT>;
     constexpr int QS = Sh::QS, ROWS = Sh::ROWS;
-    constexpr uint32_t LINE8 = D / 8 * 128;  // bytes of 8 positions (or query rows)
+    constexpr uint32_t QHALF = kRows * 128, THALF = KT * 128;  // 64 dimensions of a query tile, of a slot
     extern __shared__ __align__(1024) uint8_t smem[];
     const PagedAttnArgs &A = P.A;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -280,56 +293,61 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, ChunkShape<T, D
             const long long q_row = (long long)(q.q0 + tok0 + tok);
             const long long h_off = (long long)(head * G + h0 + row - tok * gs) * D;
             const int see = live ? p0 + tok : -1;
+            // every row of the warp sees up to here (rows that are not there see all)
+            const int see_all = __reduce_min_sync(0xffffffffu, live ? see : 0x7fffffff);
             float c = A.scale * kLog2e;
-            // ---- the warp's 32 rows to shared memory: lane (g, j) = (lane / 8, lane % 8) takes the
-            // 16-byte pieces g, g + 4, ... of rows j, j + 8, ... (8 pieces are adjacent there)
+            // ---- the warp's 32 rows to shared memory: 8 lanes take the 8 pieces of 64 dimensions
+            // of one row, 4 rows at a time
             {
-                const int g = lane >> 3, j = lane & 7;
-                uint8_t *dst0 = sq + qt * QS * Sh::QBYTES + (warp & 3) * 4 * LINE8 + j * 16 + g * 128;
-#pragma unroll 1
-                for (int i = 0; i < 4; ++i) {
-                    const int x = qt * kRows + 32 * (warp & 3) + 8 * i + j, tx = token_of(x);
-                    const bool has = x < rows;
-                    const T *src = (const T *)A.q + (long long)(q.q0 + tok0 + tx) * A.q_stride +
-                                   (long long)(head * G + h0 + x - tx * gs) * D + g * 8;
-                    uint8_t *dst = dst0 + i * LINE8;
-                    if constexpr (QS == 1) {
-                        uint4 v[D / 32];
+                const int g = lane >> 3, p = lane & 7;
+                uint8_t *const mine = sq + qt * QS * Sh::QBYTES + (warp & 3) * 32 * 128;
+                if constexpr (QS == 1) {
+#pragma unroll 4
+                    for (int i = 0; i < 8; ++i) {
+                        const int xw = 4 * i + g, x = qt * kRows + 32 * (warp & 3) + xw, tx = token_of(x);
+                        const T *src = (const T *)A.q + (long long)(q.q0 + tok0 + tx) * A.q_stride +
+                                       (long long)(head * G + h0 + x - tx * gs) * D + p * 8;
 #pragma unroll
-                        for (int k = 0; k < D / 32; ++k)
-                            v[k] = has ? *reinterpret_cast<const uint4 *>(src + k * 32) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-                        for (int k = 0; k < D / 32; ++k) *reinterpret_cast<uint4 *>(dst + k * 512) = v[k];
-                    } else {
-                        float4 v[D / 32][2];
+                        for (int h = 0; h < D / 64; ++h)
+                            *reinterpret_cast<uint4 *>(mine + h * QHALF + xw * 128 + ((p ^ (xw & 7)) * 16)) =
+                                x < rows ? *reinterpret_cast<const uint4 *>(src + h * 64) : make_uint4(0, 0, 0, 0);
+                    }
+                } else {
+#pragma unroll 2
+                    for (int i = 0; i < 8; ++i) {
+                        const int xw = 4 * i + g, x = qt * kRows + 32 * (warp & 3) + xw, tx = token_of(x);
+                        const T *src = (const T *)A.q + (long long)(q.q0 + tok0 + tx) * A.q_stride +
+                                       (long long)(head * G + h0 + x - tx * gs) * D + p * 8;
+                        float4 v[D / 64][2];
                         float most = 0.0f;
 #pragma unroll
-                        for (int k = 0; k < D / 32; ++k)
+                        for (int h = 0; h < D / 64; ++h)
 #pragma unroll
-                            for (int h = 0; h < 2; ++h)
-                                v[k][h] = has ? *reinterpret_cast<const float4 *>(src + k * 32 + h * 4) : make_float4(0, 0, 0, 0);
+                            for (int e = 0; e < 2; ++e)
+                                v[h][e] = x < rows ? *reinterpret_cast<const float4 *>(src + h * 64 + e * 4) : make_float4(0, 0, 0, 0);
 #pragma unroll
-                        for (int k = 0; k < D / 32; ++k)
+                        for (int h = 0; h < D / 64; ++h)
 #pragma unroll
-                            for (int h = 0; h < 2; ++h)
-                                most = fmaxf(most, fmaxf(fmaxf(fabsf(v[k][h].x), fabsf(v[k][h].y)),
-                                                         fmaxf(fabsf(v[k][h].z), fabsf(v[k][h].w))));
-                        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 8));
-                        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16));
+                            for (int e = 0; e < 2; ++e)
+                                most = fmaxf(most, fmaxf(fmaxf(fabsf(v[h][e].x), fabsf(v[h][e].y)),
+                                                         fmaxf(fabsf(v[h][e].z), fabsf(v[h][e].w))));
+#pragma unroll
+                        for (int d = 1; d < 8; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
                         // the row's largest value goes to [2^13, 2^14)
                         const int e = max(14, min(254, (int)(__float_as_uint(most) >> 23)));
                         const float up = __uint_as_float((uint32_t)(254 + 13 - e) << 23);
-                        const float mine = __shfl_sync(0xffffffffu, up, j);  // of row 8 i + j
-                        if (g == i) c = c / mine;
+                        const float of_row = __shfl_sync(0xffffffffu, up, (lane & 3) * 8);  // of row 4 i + lane % 4
+                        if ((lane >> 2) == i) c = c / of_row;
 #pragma unroll
-                        for (int k = 0; k < D / 32; ++k) {
+                        for (int h = 0; h < D / 64; ++h) {
                             uint4 hi, lo;
-                            split2(v[k][0].x * up, v[k][0].y * up, hi.x, lo.x);
-                            split2(v[k][0].z * up, v[k][0].w * up, hi.y, lo.y);
-                            split2(v[k][1].x * up, v[k][1].y * up, hi.z, lo.z);
-                            split2(v[k][1].z * up, v[k][1].w * up, hi.w, lo.w);
-                            *reinterpret_cast<uint4 *>(dst + k * 512) = hi;
-                            *reinterpret_cast<uint4 *>(dst + Sh::QBYTES + k * 512) = lo;
+                            split2(v[h][0].x * up, v[h][0].y * up, hi.x, lo.x);
+                            split2(v[h][0].z * up, v[h][0].w * up, hi.y, lo.y);
+                            split2(v[h][1].x * up, v[h][1].y * up, hi.z, lo.z);
+                            split2(v[h][1].z * up, v[h][1].w * up, hi.w, lo.w);
+                            uint8_t *dst = mine + h * QHALF + xw * 128 + ((p ^ (xw & 7)) * 16);
+                            *reinterpret_cast<uint4 *>(dst) = hi;
+                            *reinterpret_cast<uint4 *>(dst + Sh::QBYTES) = lo;
                         }
                     }
                 }
@@ -345,24 +363,19 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, ChunkShape<T, D
                 wait(&sfull[2 * qt + buf], (tiles_done >> 1) & 1u);
                 fence_after();
                 // ---- which of the tile's positions the row sees: bit k of word w is position 32 w + k
-                uint32_t vis[KT / 32];
-                bool all = true;
-                {
-                    const uint32_t *mk = reinterpret_cast<const uint32_t *>(marks + (tiles_done % kMarks) * (KT / 8));
-#pragma unroll
-                    for (int w = 0; w < KT / 32; ++w) {
-                        const int n = see - (tile * KT + 32 * w) + 1;
-                        vis[w] = mk[w] & (n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u);
-                        all = all && vis[w] == 0xffffffffu;
-                    }
-                    all = __all_sync(0xffffffffu, all);
-                }
+                const uint2 mk = *reinterpret_cast<const uint2 *>(marks + (tiles_done % kMarks) * (KT / 8));
+                const bool all = (mk.x & mk.y) == 0xffffffffu && tile * KT + KT - 1 <= see_all;  // warp-uniform
                 // ---- the row's scores and their maximum
                 float s[KT];
 #pragma unroll
                 for (int w = 0; w < KT / 32; ++w) tm_ld32(s_at + 32 * w, s + 32 * w);
                 wait_ld();
                 if (!all) {
+                    auto seen = [&](uint32_t m, int first) {
+                        const int n = see - first + 1;
+                        return m & (n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u);
+                    };
+                    const uint32_t vis[2] = {seen(mk.x, tile * KT), seen(mk.y, tile * KT + 32)};
 #pragma unroll
                     for (int k = 0; k < KT; ++k) s[k] = (vis[k / 32] >> (k & 31)) & 1u ? s[k] : -INFINITY;
                 }
@@ -395,7 +408,7 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, ChunkShape<T, D
                 uint64_t sum2[2] = {pair(0.0f, 0.0f), pair(0.0f, 0.0f)};
 #pragma unroll
                 for (int w = 0; w < KT / 32; ++w) {
-                    uint32_t hi[16], lo[16];
+                    uint32_t hi[16], lo[QS == 2 ? 16 : 1];
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
                         float a, b;
@@ -427,26 +440,43 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, ChunkShape<T, D
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             T *dst = (T *)A.out + q_row * A.out_stride + h_off;
             bool odd = false;
+            // whole rows pass through the warp's part of the query buffer (every product of
+            // queries is complete), 128 bytes of each at a time, so that 8 lanes store one row's;
+            // piece p of row x lies at p ^ (x & 7): no bank conflicts either way
+            uint8_t *const turn = sq + qt * QS * Sh::QBYTES + (warp & 3) * 32 * 128;
+            constexpr int PIECE = 128 / sizeof(T);  // elements of a row per round
 #pragma unroll
-            for (int d = 0; d < D; d += 32) {
-                float o[32];
-                tm_ld32(o_at + d, o);
+            for (int d = 0; d < D; d += PIECE) {
+                float o[PIECE];
+#pragma unroll
+                for (int k = 0; k < PIECE; k += 32) tm_ld32(o_at + d + k, o + k);
                 wait_ld();
 #pragma unroll
-                for (int k = 0; k < 32; ++k) odd |= (__float_as_uint(o[k]) & 0x7f800000u) == 0x7f800000u;
-                if (!live) continue;
+                for (int k = 0; k < PIECE; ++k) odd |= (__float_as_uint(o[k]) & 0x7f800000u) == 0x7f800000u;
                 if (whole) {
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) o[k] *= inv;
+                    for (int k = 0; k < PIECE; ++k) o[k] *= inv;
+                    constexpr int N = 16 / sizeof(T);
 #pragma unroll
-                    for (int k = 0; k < 32; k += 16 / sizeof(T)) {
-                        ElVec<T, 16 / sizeof(T)> v;
-                        v.set(o + k);
-                        v.store(dst + d + k);
+                    for (int p = 0; p < 8; ++p) {
+                        ElVec<T, N> v;
+                        v.set(o + p * N);
+                        v.store(reinterpret_cast<T *>(turn + lane * 128 + ((p ^ (lane & 7)) * 16)));
                     }
-                } else {
+                    __syncwarp();
 #pragma unroll
-                    for (int k = 0; k < 32; k += 4)
+                    for (int i = 0; i < 8; ++i) {
+                        const int x = 4 * i + (lane >> 3), p = lane & 7;
+                        const int xr = qt * kRows + 32 * (warp & 3) + x, tx = token_of(xr);
+                        const uint4 v = *reinterpret_cast<const uint4 *>(turn + x * 128 + ((p ^ (x & 7)) * 16));
+                        if (xr < rows)
+                            *reinterpret_cast<uint4 *>((T *)A.out + (long long)(q.q0 + tok0 + tx) * A.out_stride +
+                                                       (long long)(head * G + h0 + xr - tx * gs) * D + d + p * N) = v;
+                    }
+                    __syncwarp();
+                } else if (live) {
+#pragma unroll
+                    for (int k = 0; k < PIECE; k += 4)
                         *reinterpret_cast<float4 *>(part + ((d + k) / 4 * ROWS + row) * 4) =
                             make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
                 }
@@ -530,11 +560,16 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, ChunkShape<T, D
     } else if (warp < kIssue) {
         // ================================================================ keys and values
         const int fw = warp - 4 * QT;
-        constexpr int GRP = KT / 8 / Sh::FETCH;     // groups of 8 positions per warp
+        // A tile whose positions all exist comes by tensor copies, one box of 64 dimensions of a
+        // page's slots (or 64 of them) per copy, each completing on the slot's barrier.  The
+        // others (a sequence's end, where what lies behind it must read as zeros; pages that do
+        // not divide a tile; bad pages) come by 16-byte copies, a row's 8 pieces by 8 lanes.
+        constexpr int MINE = KT / Sh::FETCH;        // positions per warp: rows fw MINE + lane / 8 + 4 i
+        constexpr int GRP = MINE / 4;
         const uint32_t ring0 = smem_u32(ring);
-        const uint32_t my = (uint32_t)(fw * GRP) * LINE8 + (uint32_t)(lane >> 3) * 128 + (uint32_t)(lane & 7) * 16;
         int slot = 0, old = 0, pending = 0;         // next slot; the oldest not yet announced
         uint32_t lap = 0;                           // times round the ring
+        uint32_t boxed = 0, boxed_par = 0;          // slots last filled by tensor copies, their parities
         bool bad_page = false;
         auto announce = [&]() {  // the caller waited for the copies
             fence_proxy_async_smem();
@@ -543,53 +578,93 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, ChunkShape<T, D
             if (++old == P.slots) old = 0;
             --pending;
         };
+        auto drain = [&]() {
+            if (pending > 0) {
+                copies_left<0>();
+                while (pending > 0) announce();
+            }
+        };
+        const int box_rows = P.box_rows, boxes = box_rows ? KT / box_rows : 1;  // boxes of 64 dimensions
         for (; it.part(A.b); it.next(A.b)) {
             const int head = it.head / P.sets, len = it.q.len;
             const int *table = A.b.table + (long long)it.seq * A.b.table_stride;
-            auto place_of = [&](int tile, int i) { return tile * KT + (fw * GRP + i) * 8 + (lane & 7); };
-            int page[GRP];           // of the next tile's positions, read ahead
-            auto read_pages = [&](int tile) {
-#pragma unroll
-                for (int i = 0; i < GRP; ++i) {
-                    const int x = place_of(tile, i);
-                    page[i] = tile < it.tb && x < len ? __ldg(table + A.kv.page.div((uint32_t)x)) : -1;
-                }
+            // page of the tile's box `lane`, read a tile ahead
+            auto box_page = [&](int tile) {
+                const int x = tile * KT + (lane & (boxes - 1)) * box_rows;
+                return box_rows && tile < it.tb && x < len ? __ldg(table + A.kv.page.div((uint32_t)x)) : -1;
             };
-            auto offsets = [&](int tile, long long (&off)[GRP]) {  // of the lane's first piece; -1: none
-#pragma unroll
-                for (int i = 0; i < GRP; ++i) {
-                    const int x = place_of(tile, i);
-                    off[i] = -1;
-                    if (x < len) {
-                        if ((unsigned)page[i] < (unsigned)A.kv.n_pages) {
-                            const int in = x - (int)(A.kv.page.div((uint32_t)x) * A.kv.page.d);
-                            off[i] = (page[i] * A.kv.page_stride + head * A.kv.head_stride + in * A.kv.slot_stride) * (long long)sizeof(C) +
-                                     (lane >> 3) * 16;
-                        } else {
-                            bad_page = true;
-                        }
-                    }
-                    const unsigned have = __ballot_sync(0xffffffffu, off[i] >= 0);
-                    if (lane == 0) marks[(tiles_done % kMarks) * (KT / 8) + fw * GRP + i] = (uint8_t)have;
-                }
-                ++tiles_done;
+            auto mark = [&](uint32_t have, int i) {  // positions fw MINE + 4 i .. + 3, two i per byte
+                if (lane == 0) marks[(tiles_done % kMarks) * (KT / 8) + (fw * MINE + 4 * i) / 8] = (uint8_t)have;
             };
-            auto fetch = [&](const char *base, const long long (&off)[GRP]) {
+            auto boxed_tile = [&](int tile, int page) {
+                return box_rows && (tile + 1) * KT <= len && __all_sync(0xffffffffu, (unsigned)page < (unsigned)A.kv.n_pages);
+            };
+            auto claim = [&]() {  // the slot is free
                 if (lap > 0 && !bad) {
                     const uint32_t par = (lap - 1) & 1u;
                     if (!__all_sync(0xffffffffu, test_once(&empty[slot], par))) {
-                        copies_left<0>();
-                        while (pending > 0) announce();
+                        drain();
                         wait(&empty[slot], par);
                     }
                 }
+            };
+            auto fetch_boxes = [&](const void *map, int tile, int page) {
+                drain();
+                claim();
                 if (!bad) {
-                    const uint32_t dst = ring0 + (uint32_t)slot * Sh::TBYTES + my;
+                    if (fw == 0) {
+                        if (lane == 0) mbar_arrive_expect_tx(&full[slot], Sh::TBYTES);
+                        __syncwarp();
+                        const int x = tile * KT + lane * box_rows;
+                        const int in = x - (int)(A.kv.page.div((uint32_t)x) * A.kv.page.d);
+                        if (lane < boxes)
 #pragma unroll
-                    for (int i = 0; i < GRP; ++i)
+                            for (int h = 0; h < D / 64; ++h)
+                                box_load(ring0 + (uint32_t)slot * Sh::TBYTES + h * THALF + (uint32_t)(lane * box_rows) * 128, map,
+                                         h * 64, in, head, page, &full[slot]);
+                        boxed |= 1u << slot;
+                        boxed_par = (boxed_par & ~(1u << slot)) | ((lap & 1u) << slot);
+                    } else if (lane == 0) {
+                        arrive(&full[slot]);
+                    }
+                    if (++old == P.slots) old = 0;
+                }
+                if (++slot == P.slots) slot = 0, ++lap;
+            };
+            auto offsets = [&](int tile, long long (&off)[GRP]) {  // of the lane's piece; -1: none
+                uint32_t have = 0;
 #pragma unroll
-                        for (int j = 0; j < D / 32; ++j)
-                            copy16(dst + i * LINE8 + j * 512, off[i] >= 0 ? base + off[i] + j * 64 : base, off[i] >= 0);
+                for (int i = 0; i < GRP; ++i) {
+                    const int x = tile * KT + fw * MINE + 4 * i + (lane >> 3);
+                    off[i] = -1;
+                    if (x < len) {
+                        const uint32_t j = A.kv.page.div((uint32_t)x);
+                        const int page = __ldg(table + j);
+                        if ((unsigned)page < (unsigned)A.kv.n_pages)
+                            off[i] = (page * A.kv.page_stride + head * A.kv.head_stride + (x - (int)(j * A.kv.page.d)) * A.kv.slot_stride) *
+                                         (long long)sizeof(C) + (lane & 7) * 16;
+                        else bad_page = true;
+                    }
+                    const unsigned b = __ballot_sync(0xffffffffu, off[i] >= 0);  // bits 0, 8, 16, 24: rows
+                    have |= ((b & 1u) | ((b >> 7) & 2u) | ((b >> 14) & 4u) | ((b >> 21) & 8u)) << (4 * (i & 1));
+                    if (i & 1) {
+                        mark(have, i - 1);
+                        have = 0;
+                    }
+                }
+            };
+            auto fetch_rows = [&](const char *base, const long long (&off)[GRP]) {
+                claim();
+                if (!bad) {
+                    const uint32_t dst = ring0 + (uint32_t)slot * Sh::TBYTES;
+#pragma unroll
+                    for (int i = 0; i < GRP; ++i) {
+                        const int r = fw * MINE + 4 * i + (lane >> 3);
+#pragma unroll
+                        for (int h = 0; h < D / 64; ++h)
+                            copy16(dst + h * THALF + r * 128 + (((lane & 7) ^ (r & 7)) * 16), off[i] >= 0 ? base + off[i] + h * 128 : base,
+                                   off[i] >= 0);
+                    }
                     asm volatile("cp.async.commit_group;" ::: "memory");
                     if (++pending > kBehind) {
                         copies_left<kBehind>();
@@ -598,24 +673,42 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, ChunkShape<T, D
                 }
                 if (++slot == P.slots) slot = 0, ++lap;
             };
+            // K of tile ta, then K of the next tile before V of each
+            int page = box_page(it.ta), page1 = -1;
             long long off[GRP], ahead[GRP] = {};
-            read_pages(it.ta);
-            offsets(it.ta, off);
-            read_pages(it.ta + 1);
-            fetch(A.kv.k, off);
-            for (int tile = it.ta; tile < it.tb; ++tile) {
-                if (tile + 1 < it.tb) {
-                    offsets(tile + 1, ahead);
-                    read_pages(tile + 2);
-                    fetch(A.kv.k, ahead);
+            bool box = false, box1 = false;
+            auto keys = [&](int tile, int pg, long long (&o)[GRP]) {
+                const bool bx = boxed_tile(tile, pg);
+                if (bx) {
+#pragma unroll
+                    for (int i = 0; i < GRP; i += 2) mark(0xffu, i);
+                    fetch_boxes(P.map_k, tile, pg);
+                } else {
+                    offsets(tile, o);
+                    fetch_rows(A.kv.k, o);
                 }
-                fetch(A.kv.v, off);
+                ++tiles_done;
+                return bx;
+            };
+            page1 = box_page(it.ta + 1);
+            box = keys(it.ta, page, off);
+            for (int tile = it.ta; tile < it.tb; ++tile) {
+                const int page2 = box_page(tile + 2);
+                if (tile + 1 < it.tb) box1 = keys(tile + 1, page1, ahead);
+                if (box) fetch_boxes(P.map_v, tile, page);
+                else fetch_rows(A.kv.v, off);
 #pragma unroll
                 for (int i = 0; i < GRP; ++i) off[i] = ahead[i];
+                box = box1;
+                page = page1;
+                page1 = page2;
             }
         }
-        copies_left<0>();
-        while (pending > 0) announce();
+        drain();
+        // tensor copies that nothing will wait for any more, after a wait ran out
+        if (bad && fw == 0)
+            for (int i = 0; i < P.slots; ++i)
+                if ((boxed >> i) & 1u) mbar_wait_sleep(&full[i], (boxed_par >> i) & 1u, kWaitCycles / 8);
         if (__any_sync(0xffffffffu, bad_page) && lane == 0) report(A.status, TQB200_PAGED_BAD_PAGE);
     } else {
         // ================================================================ products of query tile qt
@@ -635,16 +728,16 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, ChunkShape<T, D
             wait(&full[slot], lap & 1u);
             if (!bad) {
                 fence_after();
-                const uint64_t qd = core_desc(q_at, 128, LINE8);
-                const uint64_t kd = core_desc(uniform(ring0 + (uint32_t)slot * Sh::TBYTES), 128, LINE8);
+                const uint64_t qd = row_desc(q_at, 16);
+                const uint64_t kd = row_desc(uniform(ring0 + (uint32_t)slot * Sh::TBYTES), 16);
                 const int buf = (int)uniform(scored & 1u);
                 if (one) {
 #pragma unroll
                     for (int ks = 0; ks < D / 16; ++ks)
 #pragma unroll
                         for (int sp = QS - 1; sp >= 0; --sp)
-                            mma_ss(s_of + buf * KT, qd + (sp * Sh::QBYTES + ks * 256) / 16, kd + ks * 16, id_qk,
-                                   ks > 0 || sp < QS - 1);
+                            mma_ss(s_of + buf * KT, qd + (sp * Sh::QBYTES + (ks / 4) * QHALF + (ks % 4) * 32) / 16,
+                                   kd + ((ks / 4) * THALF + (ks % 4) * 32) / 16, id_qk, ks > 0 || sp < QS - 1);
                     mma_commit(&sfull[2 * qt + buf]);
                     mma_commit(&empty[slot]);
                 }
@@ -670,7 +763,7 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, ChunkShape<T, D
                 wait(&full[slot], lap & 1u);
                 if (!bad) {
                     fence_after();
-                    const uint64_t vd = core_desc(uniform(ring0 + (uint32_t)slot * Sh::TBYTES), LINE8, 128);
+                    const uint64_t vd = row_desc(uniform(ring0 + (uint32_t)slot * Sh::TBYTES), THALF);
                     const bool more = uniform(tile > it.ta) != 0;
                     const uint32_t p_at = s_of + buf * KT;
                     if (one) {
@@ -678,7 +771,7 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, ChunkShape<T, D
                         for (int kk = 0; kk < KT / 16; ++kk)
 #pragma unroll
                             for (int sp = QS - 1; sp >= 0; --sp)
-                                mma_ts(o_at, p_at + 32 * (kk >> 1) + 8 * (kk & 1) + 16 * sp, vd + kk * 2 * (LINE8 / 16), id_pv,
+                                mma_ts(o_at, p_at + 32 * (kk >> 1) + 8 * (kk & 1) + 16 * sp, vd + kk * 2 * (1024 / 16), id_pv,
                                        kk > 0 || sp < QS - 1 || more);
                         mma_commit(&odone[2 * qt + buf]);
                         mma_commit(&empty[slot]);
@@ -703,6 +796,32 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, ChunkShape<T, D
     if (tid == 0 && s_err) report(A.status, TQB200_PAGED_TIMEOUT);
 }
 
+// Tensor map over (dimension, slot, head, page) of one of the cache's arrays, boxes of 64
+// dimensions x `rows` slots; false: it cannot be mapped.
+bool encode_pages(const char *base, const PagedAttnArgs &a, int rows, void *map128) {
+    const cuuint64_t dims[4] = {(cuuint64_t)a.head_dim, a.kv.page.d, (cuuint64_t)a.n_kv_heads, (cuuint64_t)a.kv.n_pages};
+    const long long in[3] = {a.kv.slot_stride, a.kv.head_stride, a.kv.page_stride};
+    cuuint64_t strides[3];
+    for (int i = 0; i < 3; ++i) {
+        // a dimension of one element may have any stride: a valid one in its place
+        strides[i] = (cuuint64_t)(dims[i + 1] == 1 ? a.head_dim : in[i]) * 2;
+        if (strides[i] >= (1ull << 40) || strides[i] % 16 != 0) return false;
+    }
+    const cuuint32_t box[4] = {64u, (cuuint32_t)rows, 1u, 1u}, elem[4] = {1u, 1u, 1u, 1u};
+    using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const Encode encode = reinterpret_cast<Encode>(driver_entry("cuTensorMapEncodeTiled"));
+    if (!encode) return false;
+    CUtensorMap m;
+    if (encode(&m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<char *>(base), dims, strides, box, elem,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        return false;
+    memcpy(map128, &m, sizeof(m));
+    return true;
+}
+
 template <typename T, typename C, int D, int QT>
 int launch_chunk_t(const PagedAttnArgs &a, cudaStream_t st) {
     using Sh = ChunkShape<T, D, QT>;
@@ -723,6 +842,12 @@ int launch_chunk_t(const PagedAttnArgs &a, cudaStream_t st) {
     P.g_set = (G + P.sets - 1) / P.sets;
     P.line = {Sh::ROWS / P.g_set, a.n_kv_heads * P.sets, 1, 4, 10};
     P.slots = slots;
+    // pages that a tile is made of, or that are made of tiles, in whole swizzle groups of 8 rows
+    const int page = (int)a.kv.page.d;
+    if ((page % KT == 0 || KT % page == 0) && page % 8 == 0) {
+        const int rows = std::min(page, KT);
+        if (encode_pages(a.kv.k, a, rows, P.map_k) && encode_pages(a.kv.v, a, rows, P.map_v)) P.box_rows = rows;
+    }
     const long long items = (long long)P.line.heads * (a.b.n_seqs + (long long)a.b.n_tokens / P.line.tq);
     const long long most = items * ((std::max(1, a.b.max_len) + KT - 1) / KT);
     const int grid = (int)std::min<long long>({(long long)num_sms() * Sh::CTAS, most, kSplitMaxCtas});
