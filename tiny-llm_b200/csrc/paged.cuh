@@ -346,6 +346,15 @@ __device__ __forceinline__ long long quotient(long long a, long long b) {
     return a / b;
 }
 
+// Adds 1 to a ticket, after everything that the CTA wrote (the barrier before the call puts the
+// other threads' stores before this thread's release, which is cumulative) and before everything
+// that it reads after the barrier behind the call.
+__device__ __forceinline__ unsigned take_ticket(unsigned *p) {
+    unsigned n;
+    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(n) : "l"(p) : "memory");
+    return n;
+}
+
 template <int KT>
 struct Line {
     // tiles of token block b of `nb`: positions up to its last token's, at least one tile

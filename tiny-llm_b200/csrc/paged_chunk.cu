@@ -512,12 +512,10 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, ChunkShape<T, D
             if (!whole) {
                 // ---- the last of the item's CTAs joins the parts, in order
                 const int c0 = it.first_cta(), c1 = it.last_cta();
-                __threadfence();
                 asm volatile("bar.sync 1, %0;" ::"n"(Sh::SOFT) : "memory");
-                if (tid == 0) s_last = atomicAdd(&P.tickets[c0], 1u) == (unsigned)(c1 - c0);
+                if (tid == 0) s_last = take_ticket(&P.tickets[c0]) == (unsigned)(c1 - c0);
                 asm volatile("bar.sync 1, %0;" ::"n"(Sh::SOFT) : "memory");
                 if (s_last) {
-                    __threadfence();
                     if (tid == 0) P.tickets[c0] = 0;
                     auto part_of = [&](int cta) { return P.parts + it.slot_of(cta) * ROWS * (D + 2); };
                     if (live) {

@@ -309,38 +309,52 @@ __global__ void __launch_bounds__(kThreads, kPerSm<C, D, NB>) paged_decode_kerne
             const unsigned have = __ballot_sync(0xffffffffu, off >= 0);
             off = next;
             // ---- scores: s[0], s[1] key g with columns 2t, 2t+1; s[2], s[3] key g + 8
+            // (two or three chains of sums each: the products' latency is theirs)
             float s[NB][4];
+            if constexpr (F32) {
+                float s2[NB][4], s3[NB][4];
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-                float s2[4];  // a second chain of sums: half the products' latency
+                for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[nb][e] = s2[e] = 0.0f;
+                    for (int e = 0; e < 4; ++e) s[nb][e] = s2[nb][e] = s3[nb][e] = 0.0f;
 #pragma unroll
-                for (int j = 0; j < KC; ++j) {
-                    if constexpr (F32) {
-                        const uint4 qh = q_op(0, nb, j), ql = q_op(1, nb, j);
+                for (int j = 0; j < KC; ++j)
 #pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            uint32_t hi[4], lo[4];
-                            tf32_split(__uint_as_float(word(kr[0][j], 2 * u)), hi[0], lo[0]);
-                            tf32_split(__uint_as_float(word(kr[1][j], 2 * u)), hi[1], lo[1]);
-                            tf32_split(__uint_as_float(word(kr[0][j], 2 * u + 1)), hi[2], lo[2]);
-                            tf32_split(__uint_as_float(word(kr[1][j], 2 * u + 1)), hi[3], lo[3]);
-                            mma_tf32(s2, lo, word(qh, 2 * u), word(qh, 2 * u + 1));
-                            mma_tf32(s2, hi, word(ql, 2 * u), word(ql, 2 * u + 1));
+                    for (int u = 0; u < 2; ++u) {
+                        uint32_t hi[4], lo[4];
+                        tf32_split(__uint_as_float(word(kr[0][j], 2 * u)), hi[0], lo[0]);
+                        tf32_split(__uint_as_float(word(kr[1][j], 2 * u)), hi[1], lo[1]);
+                        tf32_split(__uint_as_float(word(kr[0][j], 2 * u + 1)), hi[2], lo[2]);
+                        tf32_split(__uint_as_float(word(kr[1][j], 2 * u + 1)), hi[3], lo[3]);
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb) {
+                            const uint4 qh = q_op(0, nb, j), ql = q_op(1, nb, j);
+                            mma_tf32(s2[nb], lo, word(qh, 2 * u), word(qh, 2 * u + 1));
+                            mma_tf32(s3[nb], hi, word(ql, 2 * u), word(ql, 2 * u + 1));
                             mma_tf32(s[nb], hi, word(qh, 2 * u), word(qh, 2 * u + 1));
                         }
-                    } else {
+                    }
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[nb][e] += s2[nb][e] + s3[nb][e];
+            } else {
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                    float s2[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[nb][e] = s2[e] = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < KC; ++j)
 #pragma unroll
                         for (int sp = QS - 1; sp >= 0; --sp) {
                             const uint4 b = q_op(sp, nb, j);
                             mma16<C>(sp ? s2 : s[nb], kr[0][j].x, kr[1][j].x, kr[0][j].y, kr[1][j].y, b.x, b.y);
                             mma16<C>(QS == 1 || sp ? s2 : s[nb], kr[0][j].z, kr[1][j].z, kr[0][j].w, kr[1][j].w, b.z, b.w);
                         }
-                    }
-                }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[nb][e] += s2[e];
+                    for (int e = 0; e < 4; ++e) s[nb][e] += s2[e];
+                }
             }
             load_k(off);
             // ---- masks and the running maximum
@@ -528,12 +542,10 @@ __global__ void __launch_bounds__(kThreads, kPerSm<C, D, NB>) paged_decode_kerne
         if (!whole) {
             // ---- the item's parts from CTAs c0 .. c1; the last to arrive joins them in order
             const int c0 = it.first_cta(), c1 = it.last_cta();
-            __threadfence();
             __syncthreads();
-            if (tid == 0) s_last = atomicAdd(&P.tickets[c0], 1u) == (unsigned)(c1 - c0);
+            if (tid == 0) s_last = take_ticket(&P.tickets[c0]) == (unsigned)(c1 - c0);
             __syncthreads();
             if (s_last) {  // uniform
-                __threadfence();
                 auto part_of = [&](int cta) { return P.parts + it.slot_of(cta) * ROWS * (D + 2); };
                 constexpr int PER = ROWS * D / 4 / kThreads;  // float4 of the result per thread
                 float4 acc[PER];
