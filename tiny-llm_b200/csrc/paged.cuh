@@ -302,7 +302,9 @@ __device__ __noinline__ void row_pass(const PagedAttnArgs &A, const T *q, int se
 // the one that it ends in the middle of (slot 2c + 1).
 // Beginning an item (its queries, the first tile's latency, its results) costs as much as `over`
 // tiles, so the line counts as many units more at the front of each item.
-// Where joining (worth `join` tiles of work) would cost more than even shares save, the items
+// Joining an item's parts takes its last CTA `part` tiles for each, so an item of t tiles is not
+// cut into shares below sqrt(t part) (the least of share + parts * part).
+// Where joining at all (worth `join` tiles) would cost more than even shares save, the items
 // are taken whole instead, the sequence's last blocks (its longest) first: CTA c of g takes
 // items c, 2g - 1 - c, 2g + c, ...
 constexpr int kSplitMaxCtas = 1024;
@@ -310,7 +312,8 @@ constexpr size_t kSplitTicketBytes = kSplitMaxCtas * 4;  // head of the workspac
 
 struct LineShape {
     int tq, heads;
-    int min_quota, over, join;  // join < 0: never whole
+    int min_quota, over, join;
+    float part;  // joining one part, in tiles
 };
 
 // Sum of floor((a i + b) / m) over 0 <= i < n, a n + b < 2^32: lattice points under a line, by
@@ -451,9 +454,9 @@ struct Line {
     // sequences and of those before them.  Leaves them as items where items are taken whole.
     __device__ __forceinline__ void range(long long total, long long items, int most) {
         const long long g = gridDim.x;
-        quota = max(quotient(total + g - 1, g), (long long)sh.min_quota);
+        quota = max(quotient(total + g - 1, g), (long long)max(sh.min_quota, (int)sqrtf((float)most * sh.part)));
         most += sh.over;
-        whole = sh.join >= 0 && (items <= g ? most : quota + most / 2) <= quota + sh.join;
+        whole = (items <= g ? most : quota + most / 2) <= quota + sh.join;
         at = whole ? (long long)blockIdx.x : blockIdx.x * quota;
         end = whole ? items : min(at + quota, total);
     }

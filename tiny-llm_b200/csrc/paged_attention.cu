@@ -70,8 +70,15 @@ size_t paged_attention_work_bytes(int n_heads, int n_kv_heads, int head_dim) {
 int launch_paged_attention(const PagedAttnArgs &a, cudaStream_t st) {
     if (a.b.n_tokens == 0 || a.b.n_seqs == 0 || a.b.max_q_len == 0) return TQB200_OK;
     if (a.aligned && (a.head_dim == 64 || a.head_dim == 128)) {
+        // The tcgen05 kernel needs a 16-bit cache and pays from some work on: its items cost
+        // about 10 us before their first result.  Work is rows x positions x head_dim, the
+        // positions bounded by the page table (the lengths are known on the device only):
+        // 14 heads x 64 tokens over 564 positions (32 M) 15.1 us by mma.sync, 18.0 by tcgen05;
+        // 32 heads of 128, 64 tokens over 564 (148 M) 24.2 and 23.3; 256 over 256 (268 M) 18.2
+        // and 13.7.  Up to 16 rows of queries per KV head mma.sync reads no key twice.
         const long long rows = (long long)a.b.max_q_len * (a.n_heads / a.n_kv_heads);
-        if (a.cache_type != TQB200_EL_F32 && rows > kDecodeRows) return launch_paged_chunk(a, st);
+        const double work = (double)a.b.n_tokens * a.n_heads * a.b.max_len * a.head_dim;
+        if (a.cache_type != TQB200_EL_F32 && rows > kDecodeRows && work > 150e6) return launch_paged_chunk(a, st);
         return launch_paged_decode(a, st);
     }
     if (a.type == TQB200_EL_F32)

@@ -870,7 +870,7 @@ int launch_chunk_t(const PagedAttnArgs &a, cudaStream_t st) {
     const int G = a.n_heads / a.n_kv_heads;
     P.sets = (G + Sh::ROWS - 1) / Sh::ROWS;
     P.g_set = (G + P.sets - 1) / P.sets;
-    P.line = {Sh::ROWS / P.g_set, a.n_kv_heads * P.sets, 1, 4, 10};
+    P.line = {Sh::ROWS / P.g_set, a.n_kv_heads * P.sets, 1, 4, 10, 0.6f * QT * D / 128};
     P.slots = slots;
     // pages that a tile is made of, or that are made of tiles, in whole swizzle groups of 8 rows
     const int page = (int)a.kv.page.d;

@@ -631,7 +631,7 @@ int launch_decode_t(const PagedAttnArgs &a, cudaStream_t st) {
     const int G = a.n_heads / a.n_kv_heads;
     P.sets = (G + 8 * NB - 1) / (8 * NB);
     P.g_set = (G + P.sets - 1) / P.sets;
-    P.line = {8 * NB / P.g_set, a.n_kv_heads * P.sets, 2, 1, -1};
+    P.line = {8 * NB / P.g_set, a.n_kv_heads * P.sets, 2, 1, 2, 0.03f};
     // no more CTAs than there can be tiles
     const long long items = (long long)P.line.heads * (a.b.n_seqs + (long long)a.b.n_tokens / P.line.tq);
     const long long most = items * ((std::max(1, a.b.max_len) + kTile - 1) / kTile);
