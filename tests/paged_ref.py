@@ -15,7 +15,7 @@ class Case:
     past a sequence's pages an impossible page."""
 
     def __init__(self, new, total, heads=8, kv_heads=2, dim=64, page=16, heads_first=True, kind="f32",
-                 cache="f32", pad=0, seed=0, device="cuda", gap=0, qk=1.0, shift=0, spare=3):
+                 cache="f32", pad=0, seed=0, device="cuda", gap=0, qk=1.0, shift=0, spare=3, room=0):
         g = torch.Generator().manual_seed(seed)
         self.new, self.total, self.H, self.KVH, self.D = list(new), list(total), heads, kv_heads, dim
         self.page, self.kind, self.cache, self.dev = page, kind, cache, device
@@ -23,7 +23,9 @@ class Case:
         used = [-(-t // page) for t in total]
         self.pool = sum(used) + spare
         order = torch.randperm(self.pool, generator=g).tolist()
-        width = max(used + [1]) + 1
+        # `room`: positions that the page table has space for (a wide one sends a call with many
+        # rows to the tcgen05 kernel, which the lengths themselves do not show on the host)
+        width = max(max(used + [1]) + 1, room // page)
         self.table_cpu = torch.full((max(1, len(new)), width), 1 << 29, dtype=torch.int32)
         at = 0
         for i, u in enumerate(used):

@@ -14,6 +14,8 @@ from paged_ref import CODES, TYPES, Case, turn_tolerance, turned
 pytestmark = pytest.mark.gpu
 
 KINDS = [("f32", "f32"), ("f32", "f16"), ("f16", "f16"), ("bf16", "bf16")]
+SIXTEEN = KINDS[1:]   # caches that the tcgen05 kernel reads
+WIDE = 1 << 21        # positions of a table that is wide enough for it whatever the rows
 
 
 def near(got, want, tol, same_nan=False):
@@ -22,6 +24,8 @@ def near(got, want, tol, same_nan=False):
         assert torch.equal(got.isnan(), want.isnan())
         got, want = got[~want.isnan()], want[~want.isnan()]
     assert torch.isfinite(got).all()
+    if not got.numel():
+        return
     d = (got - want).abs()
     tol = torch.as_tensor(tol, dtype=torch.float64).expand_as(d)
     worst = (d - tol).argmax()
@@ -181,6 +185,13 @@ def test_bad_sequences_are_skipped_and_reported(tq, kind, cache, what, new):
     near(got, want, c.tolerance(most, vmax))
 
 
+@pytest.mark.parametrize("room", [0, WIDE])
+def test_rows_where_none_were_announced(tq, room):
+    c = Case([1, 2], [9, 30], 8, 2, 64, 16, True, "f16", "f16", room=room)
+    got = c.attend(tq, handles=c.handles(tq, max_q=0))
+    assert int(c.status) == tq.PAGED_BAD_SEQ and bool((got == 7.0).all())
+
+
 @pytest.mark.parametrize("kind,cache", KINDS)
 @pytest.mark.parametrize("new", [1, 90])
 def test_calls_repeat_bit_for_bit_and_leave_the_workspace_ready(tq, kind, cache, new):
@@ -281,6 +292,123 @@ def test_matches_the_contiguous_decode_attention(tq):
     got = c.attend(tq).cpu().numpy().reshape(-1)
     _, m, vmax = c.want()
     assert np.abs(got - want).max() <= 2 * c.tolerance(m, vmax)
+
+
+# ------------------------------------------------------------------ the tcgen05 kernel on small cases
+@pytest.mark.parametrize("kind,cache", SIXTEEN)
+@pytest.mark.parametrize("H,KVH,D", SHAPES + [(130, 1, 64), (300, 1, 128)])
+@pytest.mark.parametrize("page,first", [(16, False), (24, True), (1, True), (64, True), (128, False), (8, True)])
+def test_chunks_on_tcgen05(tq, kind, cache, H, KVH, D, page, first):
+    new, total = [37, 1, 130, 17], [37, 90, 261, 64]
+    c = Case(new, total, H, KVH, D, page, first, kind, cache, pad=1, seed=page + H, room=WIDE)
+    check(c, tq)
+    assert int(c.status) == 0
+
+
+@pytest.mark.parametrize("kind,cache", SIXTEEN)
+@pytest.mark.parametrize("new,total", [
+    ([0, 20, 0, 40], [0, 29, 12, 60]), ([50, 30], [20, 0]), ([17, 0, 0], [0, 0, 0]), ([200, 17], [100, 17]),
+    ([64], [64]), ([64], [128]), ([65], [129]), ([63], [65]), ([300], [300])])
+def test_lengths_on_tcgen05(tq, kind, cache, new, total):
+    c = Case(new, total, 8, 2, 128, 16, True, kind, cache, pad=3, seed=5, room=WIDE)
+    got = check(c, tq)
+    assert torch.equal(got[sum(new):].float(), torch.full_like(got[sum(new):].float(), 7.0))
+
+
+@pytest.mark.parametrize("kind,cache", SIXTEEN)
+@pytest.mark.parametrize("gap,qk", [(8, 1.0), (64, 1.0), (0, 4.0)])
+def test_strides_and_large_scores_on_tcgen05(tq, kind, cache, gap, qk):
+    c = Case([100, 40], [300, 60], 8, 2, 64, 16, True, kind, cache, gap=gap, qk=qk, seed=9, room=WIDE)
+    check(c, tq)
+    rows = c.obuf[:c.n * c.qw].view(c.n, c.qw)
+    assert bool((rows[:, c.H * c.D:] == 7.0).all()) and bool((c.obuf[c.n * c.qw:] == 7.0).all())
+
+
+@pytest.mark.parametrize("kind,cache", SIXTEEN)
+@pytest.mark.parametrize("new,total,x", [(150, 200, 120), (150, 200, 199), (130, 700, 571), (20, 900, 30)])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("what", [math.nan, math.inf])
+def test_non_finite_values_on_tcgen05(tq, kind, cache, new, total, x, D, what):
+    c = Case([new], [total], 8, 2, D, 16, True, kind, cache, seed=x, room=WIDE)
+    want, most, vmax = c.want()
+    p = int(c.table_cpu[0, x // 16])
+    c.kview[p, 0, x % 16, 5] = what
+    c.vview[p, 0, x % 16, 7] = what
+    c.upload()
+    got = c.attend(tq).double().cpu()
+    torch.cuda.synchronize()
+    blind = max(0, x - (total - new))
+    near(got[:blind], want[:blind], c.tolerance(most, vmax))
+    half = 4 * D
+    near(got[:, half:], want[:, half:], c.tolerance(most, vmax))
+    assert not torch.isfinite(got[blind:, 7]).all()
+
+
+@pytest.mark.parametrize("kind,cache", SIXTEEN)
+@pytest.mark.parametrize("page_id", [-1, 1 << 30])
+def test_bad_pages_and_sequences_on_tcgen05(tq, kind, cache, page_id):
+    c = Case([70, 20, 30], [290, 33, 90], 8, 2, 64, 16, True, kind, cache, seed=4, room=WIDE)
+    c.table_cpu[0, 1] = page_id
+    c.upload()
+    drop = {(0, x) for x in range(16, 32)}
+    check(c, tq, drop=drop)
+    assert int(c.status) == tq.PAGED_BAD_PAGE
+    want, most, vmax = c.want(drop)
+    c.obuf.fill_(7.0)
+    c.status.zero_()
+    c.len[1] = -1
+    got = c.attend(tq).double().cpu()
+    want[70:90] = 7.0
+    near(got, want, c.tolerance(most, vmax))
+    assert int(c.status) in (tq.PAGED_BAD_SEQ, tq.PAGED_BAD_PAGE)
+
+
+@pytest.mark.parametrize("kind,cache", SIXTEEN)
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_prompt_from_its_beginning(tq, kind, cache, D):
+    """Whole items, one query tile each: a table with room for the prompt only."""
+    c = Case([400, 211], [400, 230], 16, 4, D, 16, True, kind, cache, seed=D)
+    check(c, tq)
+
+
+@pytest.mark.parametrize("kind,cache", SIXTEEN)
+def test_tcgen05_calls_repeat_and_follow_a_graph(tq, kind, cache):
+    """Items split over CTAs and joined: bit for bit the same every time, whatever other call used
+    the workspace in between; captured and replayed with other lengths."""
+    c = Case([90, 60, 17], [2500, 700, 3000], 8, 2, 128, 16, True, kind, cache, seed=8, room=WIDE)
+    h = c.handles(tq)
+    w = c.workspace(tq, *h)
+    first = check(c, tq, work=w, handles=h).clone()
+    other = Case([1, 1], [1000, 1500], 8, 2, 64, 16, True, kind, cache, seed=1)
+    for _ in range(4):
+        c.obuf.fill_(7.0)
+        assert torch.equal(c.attend(tq, work=w, handles=h), first)
+        check(other, tq, work=w)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        c.attend(tq, work=w, handles=h)
+    for lens in ([2500, 700, 3000], [90, 500, 17], [1111, 60, 2999]):
+        c.total = lens
+        c.len.copy_(torch.tensor(lens, dtype=torch.int32))
+        c.obuf.fill_(7.0)
+        g.replay()
+        torch.cuda.synchronize()
+        want, most, vmax = c.want()
+        near(c.out(), want, c.tolerance(most, vmax))
+
+
+@pytest.mark.parametrize("kind,cache", KINDS)
+@pytest.mark.parametrize("seqs,new", [(33, 1), (150, 1), (300, 1), (40, 6), (140, 3)])
+def test_many_sequences(tq, kind, cache, seqs, new):
+    """More sequences than a warp's lanes, than a CTA's threads; some without rows."""
+    new = [0 if i % 7 == 3 else new for i in range(seqs)]
+    total = [n + (i * 37) % 90 for i, n in enumerate(new)]
+    for room in (0, WIDE):
+        c = Case(new, total, 8, 2, 64, 16, True, kind, cache, pad=1, seed=seqs, room=room)
+        check(c, tq)
+        assert int(c.status) == 0
 
 
 # ------------------------------------------------------------------ norms and rotation

@@ -68,7 +68,7 @@ size_t paged_attention_work_bytes(int n_heads, int n_kv_heads, int head_dim) {
 }
 
 int launch_paged_attention(const PagedAttnArgs &a, cudaStream_t st) {
-    if (a.b.n_tokens == 0 || a.b.n_seqs == 0 || a.b.max_q_len == 0) return TQB200_OK;
+    if (a.b.n_tokens == 0 || a.b.n_seqs == 0) return TQB200_OK;
     if (a.aligned && (a.head_dim == 64 || a.head_dim == 128)) {
         // The tcgen05 kernel needs a 16-bit cache and pays from some work on: its items cost
         // about 10 us before their first result.  Work is rows x positions x head_dim, the
