@@ -399,6 +399,18 @@ def test_tcgen05_calls_repeat_and_follow_a_graph(tq, kind, cache):
         near(c.out(), want, c.tolerance(most, vmax))
 
 
+@pytest.mark.parametrize("cache,room,new", [("f16", WIDE, 64), ("f16", 0, 1), ("f32", 0, 1), ("f32", 0, 20)])
+def test_fp32_results_keep_their_precision_over_long_contexts(tq, cache, room, new):
+    """Tensor-core sums are cut, not rounded, so an error that grows with the context shows in the
+    2-norm.  Bound: sums of at most 8 tiles of 8 products, each cut by less than 2^-24 of the sum
+    (64), the scores' 16 products likewise, splits to 2^-21 twice, and as much again for what
+    fp32 additions round at random: 2 * (80 * 2^-24 + 2 * 2^-21) / 2 on average half of it."""
+    c = Case([new], [12000], 2, 1, 128, 16, True, "f32", cache, qk=1.0, seed=1, room=room)
+    got = c.attend(tq).double().cpu()
+    want, _, _ = c.want()
+    assert float((got - want).norm() / want.norm()) <= 80 * 2.0 ** -24 + 2 * 2.0 ** -21
+
+
 @pytest.mark.parametrize("kind,cache", KINDS)
 @pytest.mark.parametrize("seqs,new", [(33, 1), (150, 1), (300, 1), (40, 6), (140, 3)])
 def test_many_sequences(tq, kind, cache, seqs, new):

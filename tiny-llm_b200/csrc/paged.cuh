@@ -58,7 +58,7 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
 // N consecutive elements as one load or store of N * sizeof(T) <= 16 bytes (N = 8 fp32: two).
 template <typename T, int N>
 struct ElVec {
-    static_assert(N * sizeof(T) <= 16 || N * sizeof(T) == 32, "vector size");
+    static_assert(N * sizeof(T) == 8 || N * sizeof(T) == 16 || N * sizeof(T) == 32, "vector size");
     static constexpr int W = N * sizeof(T) / 4;
     uint32_t w[W];
     __device__ __forceinline__ void load(const T *p) {
@@ -68,11 +68,9 @@ struct ElVec {
                 const uint4 v = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint32_t *>(p) + i);
                 w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
             }
-        } else if constexpr (W == 2) {
+        } else {
             const uint2 v = *reinterpret_cast<const uint2 *>(p);
             w[0] = v.x, w[1] = v.y;
-        } else {
-            w[0] = *reinterpret_cast<const uint32_t *>(p);
         }
     }
     __device__ __forceinline__ void store(T *p) const {
@@ -81,19 +79,8 @@ struct ElVec {
             for (int i = 0; i < W; i += 4)
                 *reinterpret_cast<uint4 *>(reinterpret_cast<uint32_t *>(p) + i) =
                     make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
-        } else if constexpr (W == 2) {
-            *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
         } else {
-            *reinterpret_cast<uint32_t *>(p) = w[0];
-        }
-    }
-    __device__ __forceinline__ float get(int i) const {
-        if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
-        else {
-            const uint16_t b = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
-            T t;
-            memcpy(&t, &b, 2);
-            return el_to_f<T>(t);
+            *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
         }
     }
     // elements 2 i and 2 i + 1

@@ -8,8 +8,9 @@
 //   O += P V (128 x D, fp32 in TMEM), P as the A operand from TMEM.
 // Bound: the tensor pipe for long chunks (4 D operations per row, key and value).  Beside it
 // runs one exponential per score on 16 lanes per clock, which takes as long as the products
-// of 16-bit operands (128 x 128 scores: 1024 clocks either way), so two query tiles alternate:
-// while one is in its softmax the other's products run.
+// of 16-bit operands (128 x 64 scores of D 128: 512 clocks either way), so two query tiles
+// alternate and each has two score buffers: the next tile's scores are formed while this one's
+// softmax runs.
 // Roles (warps): QT groups of 4 softmax warps (thread = query row = TMEM lane), 2 QT warps that
 // fetch keys and values, QT warps that each issue one query tile's products.
 //  * A ring of slots holds whole K or V tiles in the order they are used, K0 K1 V0 K2 V1 ...
@@ -25,6 +26,17 @@
 //    split into fp16 hi + lo, two products each: 22 bits of either operand.
 //  * Every wait is bounded; after one runs out the roles go on without waiting or issuing, the
 //    issued copies and products are waited for (bounded), TMEM is freed and the error stored.
+//
+// Measured on one B200 (device time): 2048 rows of 32 heads over 8 KV heads of 128 and 16384
+// bf16 positions (515 GFLOP) 500 to 540 us by the clock's state, 0.95 to 1.03 PFLOP/s; 512 rows
+// of 32 heads over 4 KV heads, fp32 over fp16, 23.6 us.  What it came from, at the first shape:
+// 861 us with a thread's own descriptors for every MMA (96 to 130 clocks each to issue, against
+// 64 now), 720 with one score buffer of 128 keys, 640 with two of 64, 519 with tiles by TMA
+// instead of 16-byte copies (without any copies it took 529 then: the copies were the bound).
+// Taking a quarter of the exponentials to a polynomial on the FMA pipe, or letting the two
+// query tiles take turns at the exponential, changed nothing.  A tile of 64 keys takes about
+// 2400 clocks for both query tiles, of which the products need 1280; the softmax warps' own
+// chain (TMEM load, maximum, exponential, TMEM store) is what is left.
 #include <cuda.h>
 #include <string.h>
 
@@ -38,6 +50,7 @@ namespace {
 
 constexpr float kRaise = 8.0f;
 constexpr float kLift = 6.0f;
+constexpr int kFold = 8;          // tiles per sum in TMEM where results are fp32
 constexpr int kBehind = 3;        // tiles whose copies a fetching warp leaves in flight
 constexpr int kRows = 128;        // query rows per tile: TMEM lanes
 constexpr int kMaxSlots = 12;
@@ -50,6 +63,7 @@ struct ChunkParams {
     PagedAttnArgs A;
     unsigned *tickets;
     float *parts;     // [2 grid]: [D / 4][rows][4] accumulators, [rows] maxima, [rows] sums
+    float *kept;      // [grid][D / 4][rows][4]: sums of earlier tiles (fp32 results)
     LineShape line;
     int sets, g_set;
     int slots;
@@ -357,8 +371,36 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, ChunkShape<T, D
                 __syncwarp();
                 if (lane == 0) arrive(&qready[qt]);
             }
-            float m = -INFINITY, l = 0.0f;
+            float m = -INFINITY, l = 0.0f, m_kept = -INFINITY;
+            float *const kept = P.kept + ((long long)blockIdx.x * ROWS * D + row * 4);
             for (int tile = it.ta; tile < it.tb; ++tile, ++tiles_done) {
+                // A tensor-core sum is cut, not rounded, at every product: over 12000 positions the results
+                // came out 6e-6 short.  For fp32 results the sums start anew every kFold tiles, and what
+                // they reached is added to a copy in the workspace, which this thread alone touches.
+                const bool fold = QS == 2 && tile > it.ta && (tile - it.ta) % kFold == 0;
+                if (fold) {
+                    wait_product(tiles_done - 1);
+                    fence_after();
+                    const bool first = tile - it.ta == kFold;
+                    const float f = first || m_kept == -INFINITY ? 0.0f : ex2(m_kept - m);
+                    m_kept = m;
+#pragma unroll 1
+                    for (int d = 0; d < D; d += 32) {
+                        float o[32];
+                        tm_ld32(o_at + d, o);
+                        float4 x[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            x[k] = first ? make_float4(0, 0, 0, 0) : *reinterpret_cast<const float4 *>(kept + ((d / 4 + k) * ROWS) * 4);
+                        wait_ld();
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            *reinterpret_cast<float4 *>(kept + ((d / 4 + k) * ROWS) * 4) =
+                                make_float4(fmaf(f, x[k].x, o[4 * k]), fmaf(f, x[k].y, o[4 * k + 1]), fmaf(f, x[k].z, o[4 * k + 2]),
+                                            fmaf(f, x[k].w, o[4 * k + 3]));
+                    }
+                    fence_before();
+                }
                 const int buf = tiles_done & 1;
                 const uint32_t s_at = s_of + (uint32_t)(buf * KT);
                 wait(&sfull[2 * qt + buf], (tiles_done >> 1) & 1u);
@@ -389,7 +431,7 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, ChunkShape<T, D
                     const float f = raise ? ex2(m - mx) : 1.0f;  // 0 from -inf
                     if (raise) m = mx;
                     l *= f;
-                    if (tile > it.ta) {  // O holds something, once the product before is complete
+                    if (tile > it.ta && !fold) {  // O holds something, once the product before is complete
                         wait_product(tiles_done - 1);
                         fence_after();
 #pragma unroll 1
@@ -452,6 +494,15 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, ChunkShape<T, D
 #pragma unroll
                 for (int k = 0; k < PIECE; k += 32) tm_ld32(o_at + d + k, o + k);
                 wait_ld();
+                if (QS == 2 && it.tb - it.ta > kFold) {
+                    const float f = m_kept == -INFINITY ? 0.0f : ex2(m_kept - m);
+#pragma unroll
+                    for (int k = 0; k < PIECE; k += 4) {
+                        const float4 x = *reinterpret_cast<const float4 *>(kept + ((d + k) / 4 * ROWS) * 4);
+                        o[k] = fmaf(f, x.x, o[k]), o[k + 1] = fmaf(f, x.y, o[k + 1]);
+                        o[k + 2] = fmaf(f, x.z, o[k + 2]), o[k + 3] = fmaf(f, x.w, o[k + 3]);
+                    }
+                }
 #pragma unroll
                 for (int k = 0; k < PIECE; ++k) odd |= (__float_as_uint(o[k]) & 0x7f800000u) == 0x7f800000u;
                 if (whole) {
@@ -763,9 +814,9 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, ChunkShape<T, D
                 const int buf = (int)uniform(scored & 1u);
                 if (one) {
 #pragma unroll
-                    for (int ks = 0; ks < D / 16; ++ks)
+                    for (int sp = QS - 1; sp >= 0; --sp)  // the small terms first: less is cut from them
 #pragma unroll
-                        for (int sp = QS - 1; sp >= 0; --sp)
+                        for (int ks = 0; ks < D / 16; ++ks)
                             mma_ss(s_of + buf * KT, qd + (sp * Sh::QBYTES + (ks / 4) * QHALF + (ks % 4) * 32) / 16,
                                    kd + ((ks / 4) * THALF + (ks % 4) * 32) / 16, id_qk, ks > 0 || sp < QS - 1);
                     mma_commit(&sfull[2 * qt + buf]);
@@ -794,7 +845,7 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, ChunkShape<T, D
                 if (!bad) {
                     fence_after();
                     const uint64_t vd = row_desc(uniform(ring0 + (uint32_t)slot * Sh::TBYTES), THALF);
-                    const bool more = uniform(tile > it.ta) != 0;
+                    const bool more = uniform(tile > it.ta && !(QS == 2 && (tile - it.ta) % kFold == 0)) != 0;
                     const uint32_t p_at = s_of + buf * KT;
                     if (one) {
 #pragma unroll
@@ -825,6 +876,9 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, ChunkShape<T, D
     }
     if (tid == 0 && s_err) report(A.status, TQB200_PAGED_TIMEOUT);
 }
+
+// Two parts for each of the grid's CTAs, 256 rows of them per SM.
+size_t parts_floats(int head_dim) { return (size_t)std::min(4 * num_sms(), 2 * kSplitMaxCtas) * kRows * (size_t)(head_dim + 2); }
 
 // Tensor map over (dimension, slot, head, page) of one of the cache's arrays, boxes of 64
 // dimensions x `rows` slots; false: it cannot be mapped.
@@ -867,6 +921,7 @@ int launch_chunk_t(const PagedAttnArgs &a, cudaStream_t st) {
     P.A = a;
     P.tickets = (unsigned *)a.work;
     P.parts = (float *)((char *)a.work + kSplitTicketBytes);
+    P.kept = P.parts + parts_floats(D);
     const int G = a.n_heads / a.n_kv_heads;
     P.sets = (G + Sh::ROWS - 1) / Sh::ROWS;
     P.g_set = (G + P.sets - 1) / P.sets;
@@ -900,8 +955,7 @@ int launch_chunk_c(const PagedAttnArgs &a, cudaStream_t st) {
 }  // namespace
 
 size_t paged_chunk_work_bytes(int head_dim) {
-    const size_t slots = std::min(4 * num_sms(), 2 * kSplitMaxCtas);  // 2 per CTA of 128 rows: 2 CTAs per SM
-    return kSplitTicketBytes + slots * kRows * (size_t)(head_dim + 2) * 4;
+    return kSplitTicketBytes + parts_floats(head_dim) * 4 + (size_t)num_sms() * 2 * kRows * head_dim * 4;
 }
 
 int launch_paged_chunk(const PagedAttnArgs &a, cudaStream_t st) {
