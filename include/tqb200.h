@@ -293,7 +293,7 @@ int tqb200_dev_qk_norm_rope(const void *q, const void *k, void *q_out, void *k_o
  * queries) and k and v into the cache's pages, in one launch.  The rotation uses
  * positions[row], or the row's cache position when positions is NULL.  Rows whose cache
  * position is negative (kv_len below the sequence's new rows) are not stored.  Two rows that
- * map to one slot (a page listed twice) race: either may end up there. */
+ * map to one slot (a page listed twice) race: the slot may end up with parts of either. */
 int tqb200_dev_paged_append(const void *q, const void *k, const void *v, void *q_out, int type,
                             int n_heads, int rotary_dim, long long q_stride, long long k_stride,
                             long long v_stride, long long q_out_stride, const float *q_norm,

@@ -26,12 +26,15 @@
 // flight while the present ones are used; page numbers are read one step further ahead.
 //
 // Measured on one B200 (device time): 64 single tokens of 32 heads over 8 KV heads of 128, 126
-// thousand bf16 positions (516 MB): 86 us, 6.0 TB/s of the 6.5 of a copy; one token over 4096
-// fp16 positions (16.8 MB) 14.7 us, of which planning takes 1.4, the queries and first keys
+// thousand bf16 positions (516 MB): 88 us, 5.9 TB/s of the 6.5 of a copy; one token over 4096
+// fp16 positions (16.8 MB) 15.6 us, of which planning takes 1.4, the queries and first keys
 // 2.4, two steps of 64 keys 2.6, the join of 33 parts 4.5; 3 tokens over up to 40 fp32
-// positions 5.1 us.  With one chain of sums for the scores a step took 530 clocks longer; with
-// the planning in 64-bit divisions and two barriers every call took 4 us longer.  Over an fp32
-// cache a chunk of 2000 rows over 8000 positions takes 5.4 ms (42 TFLOP/s): three tf32 products per term, and each block of 16 rows reads the
+// positions 6.0 us.  With one chain of sums for the scores a step took 530 clocks longer; with
+// the planning in 64-bit divisions and two barriers every call took 4 us longer.  Where results
+// are fp32, each step's sums start at zero in the tensor core and are added to the accumulators
+// in fp32: the tensor core cuts its sums, which over 12000 positions came to 6e-6.  Over an
+// fp32 cache a chunk of 2000 rows of 32 heads over up to 8000 positions takes 6.6 ms (5.4 with
+// running sums), 35 TFLOP/s: three tf32 products per term, and each block of 16 rows reads the
 // cache again from L2.
 #include <algorithm>
 #include <type_traits>
