@@ -306,6 +306,17 @@ def test_chunks_on_tcgen05(tq, kind, cache, H, KVH, D, page, first):
 
 
 @pytest.mark.parametrize("kind,cache", SIXTEEN)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("page,first", [(40, False), (48, True), (96, False), (192, True), (72, True)])
+def test_pages_that_tiles_do_not_divide_on_tcgen05(tq, kind, cache, D, page, first):
+    """Pages that begin and end inside a tile of 64 positions."""
+    new, total = [33, 1, 70, 20], [400, 257, 641, 192]
+    c = Case(new, total, 8, 2, D, page, first, kind, cache, pad=1, seed=page + D, room=WIDE)
+    check(c, tq)
+    assert int(c.status) == 0
+
+
+@pytest.mark.parametrize("kind,cache", SIXTEEN)
 @pytest.mark.parametrize("new,total", [
     ([0, 20, 0, 40], [0, 29, 12, 60]), ([50, 30], [20, 0]), ([17, 0, 0], [0, 0, 0]), ([200, 17], [100, 17]),
     ([64], [64]), ([64], [128]), ([65], [129]), ([63], [65]), ([300], [300])])

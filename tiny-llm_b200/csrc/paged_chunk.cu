@@ -44,6 +44,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <numeric>
 #include <type_traits>
 
 #include "paged.cuh"
@@ -683,20 +684,23 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, ChunkShape<T, D
                 drain();
                 claim();
                 if (!bad) {
-                    if (fw == 0) {
-                        if (lane == 0) mbar_arrive_expect_tx(&full[slot], Sh::TBYTES);
-                        __syncwarp();
-                        const int x = tile * KT + lane * box_rows;
-                        const int in = x - (int)(A.kv.page.div((uint32_t)x) * A.kv.page.d);
-                        if (lane < boxes)
-#pragma unroll
-                            for (int h = 0; h < D / 64; ++h)
-                                box_load(ring0 + (uint32_t)slot * Sh::TBYTES + h * THALF + (uint32_t)(lane * box_rows) * 128, map,
-                                         h * 64, in, head, page, &full[slot]);
+                    // copy j of boxes x D / 64 by warp j % FETCH: a thread issues them one by one
+                    constexpr int H = D / 64;
+                    const int mine = (boxes * H - fw + Sh::FETCH - 1) / Sh::FETCH;
+                    if (lane == 0) {
+                        if (mine > 0) mbar_arrive_expect_tx(&full[slot], (uint32_t)(mine * box_rows) * 128);
+                        else arrive(&full[slot]);
+                    }
+                    __syncwarp();
+                    const int j = fw + lane * Sh::FETCH, i = j / H, h = j % H;
+                    const int at = __shfl_sync(0xffffffffu, page, i & 31);
+                    const int x = tile * KT + i * box_rows;
+                    if (lane < mine)
+                        box_load(ring0 + (uint32_t)slot * Sh::TBYTES + h * THALF + (uint32_t)(i * box_rows) * 128, map, h * 64,
+                                 x - (int)(A.kv.page.div((uint32_t)x) * A.kv.page.d), head, at, &full[slot]);
+                    if (mine > 0) {
                         boxed |= 1u << slot;
                         boxed_par = (boxed_par & ~(1u << slot)) | ((lap & 1u) << slot);
-                    } else if (lane == 0) {
-                        arrive(&full[slot]);
                     }
                     if (++old == P.slots) old = 0;
                 }
@@ -790,7 +794,7 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, ChunkShape<T, D
         }
         drain();
         // tensor copies that nothing will wait for any more, after a wait ran out
-        if (bad && fw == 0)
+        if (bad)
             for (int i = 0; i < P.slots; ++i)
                 if ((boxed >> i) & 1u) mbar_wait_sleep(&full[i], (boxed_par >> i) & 1u, kWaitCycles / 8);
         if (__any_sync(0xffffffffu, bad_page) && lane == 0) report(A.status, TQB200_PAGED_BAD_PAGE);
@@ -930,10 +934,9 @@ int launch_chunk_t(const PagedAttnArgs &a, cudaStream_t st) {
     P.g_set = (G + P.sets - 1) / P.sets;
     P.line = {Sh::ROWS / P.g_set, a.n_kv_heads * P.sets, 1, 4, 10, 0.6f * QT * D / 128};
     P.slots = slots;
-    // pages that a tile is made of, or that are made of tiles, in whole swizzle groups of 8 rows
-    const int page = (int)a.kv.page.d;
-    if ((page % KT == 0 || KT % page == 0) && page % 8 == 0) {
-        const int rows = std::min(page, KT);
+    // boxes that lie in one page and start on the swizzle's groups of 8 rows
+    const int rows = std::gcd((int)a.kv.page.d, KT);
+    if (rows % 8 == 0) {
         if (encode_pages(a.kv.k, a, rows, P.map_k) && encode_pages(a.kv.v, a, rows, P.map_v)) P.box_rows = rows;
     }
     const long long items = (long long)P.line.heads * (a.b.n_seqs + (long long)a.b.n_tokens / P.line.tq);

@@ -234,8 +234,10 @@ def _stream(stream):
         except Exception:
             return None
         # the same handle without a Stream object per call (3.7 us down to 0.4)
-        raw, current = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
-        _torch_stream = lambda: raw(current())  # noqa: E731
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        current = getattr(torch._C, "_cuda_getDevice", None)
+        if raw and current:
+            _torch_stream = lambda: raw(current())  # noqa: E731
         return handle
     return stream
 
