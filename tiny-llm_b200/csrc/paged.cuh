@@ -303,31 +303,20 @@ struct LineShape {
     float part;  // joining one part, in tiles
 };
 
-// Sum of floor((a i + b) / m) over 0 <= i < n, a n + b < 2^32: lattice points under a line, by
-// exchanging the axes as in Euclid's algorithm (Graham, Knuth, Patashnik, Concrete
-// Mathematics, 3.5).  With a, b < m the line reaches height h = floor((a (n-1) + b) / m); the
-// points (i, y), 1 <= y <= h, under it are, per y, those with i >= (m y - b) / a:
-// n h - sum_y ceil((m y - b) / a), and ceil((m y - b) / a) = floor((m (y - 1) + m - b + a - 1) / a).
-__device__ inline long long floor_line_sum(uint32_t n, uint32_t a, uint32_t b, uint32_t m) {
-    long long sum = 0, sign = 1;
-    while (n > 0) {
-        if (a >= m || b >= m) {
-            const uint32_t qa = a / m, qb = b / m;
-            sum += sign * ((long long)qa * ((long long)n * (n - 1) / 2) + (long long)qb * n);
-            a -= qa * m;
-            b -= qb * m;
-        }
-        const uint32_t h = (a * (n - 1) + b) / m;
-        if (h == 0) break;
-        sum += sign * (long long)n * h;
-        sign = -sign;
-        const uint32_t b2 = m - b + a - 1, m2 = a;
-        n = h;
-        b = b2;
-        a = m;
-        m = m2;
-    }
-    return sum;
+// Sum of floor((a i + b) / M) over 0 <= i < n, M a power of two, a > 0: a i + b less its residue,
+// over M.  The residues repeat every M / g terms, g = gcd(a, M), and are b mod g + 0, g, 2 g, ...
+// in some order; the terms behind the last whole round are added up.
+template <int M>
+__device__ inline long long floor_line_sum(uint32_t n, uint32_t a, uint32_t b) {
+    static_assert((M & (M - 1)) == 0, "power of two");
+    const uint32_t g = min((uint32_t)M, a & (0u - a)), shift = __ffs(g) - 1, per = (uint32_t)M >> shift;
+    const uint32_t rest = n & (per - 1), round = per * (b & (g - 1)) + g * (per * (per - 1) / 2);
+    uint32_t tail = 0;
+#pragma unroll 4
+    for (uint32_t i = 0; i < rest; ++i) tail += (a * i + b) & (M - 1);
+    const unsigned long long all = (unsigned long long)n * (n - 1) / 2 * a + (unsigned long long)n * b;
+    const unsigned long long residues = (unsigned long long)(n / per) * round + tail;
+    return (long long)((all - residues) / M);
 }
 
 // a / b, mostly of 32-bit values
@@ -362,8 +351,8 @@ struct Line {
             const int p0 = q.len - q.n;
             // the blocks before it: those that end before position 0 have one tile each
             const int none = p0 < 0 ? min(nb - 1, (int)((uint32_t)(-p0) / (uint32_t)tq)) : 0;
-            sum += nb - 1 + floor_line_sum((uint32_t)(nb - 1 - none), (uint32_t)tq,
-                                           (uint32_t)((long long)p0 + (long long)none * tq + tq - 1), KT);
+            sum += nb - 1 + floor_line_sum<KT>((uint32_t)(nb - 1 - none), (uint32_t)tq,
+                                               (uint32_t)((long long)p0 + (long long)none * tq + tq - 1));
         }
         return sum;
     }

@@ -332,6 +332,7 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, ChunkShape<T, D
                                 x < rows ? *reinterpret_cast<const uint4 *>(src + h * 64) : make_uint4(0, 0, 0, 0);
                     }
                 } else {
+                    float scaled = 1.0f;  // this lane's row
 #pragma unroll 4
                     for (int i = 0; i < 8; ++i) {
                         const int xw = 4 * i + g, x = qt * kRows + 32 * (warp & 3) + xw, tx = token_of(x);
@@ -356,7 +357,7 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, ChunkShape<T, D
                         const int e = max(14, min(254, (int)(__float_as_uint(most) >> 23)));
                         const float up = __uint_as_float((uint32_t)(254 + 13 - e) << 23);
                         const float of_row = __shfl_sync(0xffffffffu, up, (lane & 3) * 8);  // of row 4 i + lane % 4
-                        if ((lane >> 2) == i) c = c / of_row;
+                        scaled = (lane >> 2) == i ? of_row : scaled;
 #pragma unroll
                         for (int h = 0; h < D / 64; ++h) {
                             uint4 hi, lo;
@@ -369,6 +370,7 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, ChunkShape<T, D
                             *reinterpret_cast<uint4 *>(dst + Sh::QBYTES) = lo;
                         }
                     }
+                    c = c / scaled;
                 }
                 fence_proxy_async_smem();
                 fence_before();  // the previous item's reads of O are complete
@@ -486,7 +488,7 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, ChunkShape<T, D
             float *part = P.parts + it.slot_of(blockIdx.x) * ROWS * (D + 2);
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             T *dst = (T *)A.out + q_row * A.out_stride + h_off;
-            bool odd = false;
+            uint64_t naught[2] = {pair(0.0f, 0.0f), pair(0.0f, 0.0f)};  // NaN once a value is not finite
             // whole rows pass through the warp's part of the query buffer (every product of
             // queries is complete), 128 bytes of each at a time, so that 8 lanes store one row's;
             // piece p of row x lies at p ^ (x & 7): no bank conflicts either way
@@ -508,10 +510,11 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, ChunkShape<T, D
                     }
                 }
 #pragma unroll
-                for (int k = 0; k < PIECE; ++k) odd |= (__float_as_uint(o[k]) & 0x7f800000u) == 0x7f800000u;
+                for (int k = 0; k < PIECE; k += 2)
+                    naught[(k / 2) & 1] = fma2(pair(o[k], o[k + 1]), pair(0.0f, 0.0f), naught[(k / 2) & 1]);
                 if (whole) {
 #pragma unroll
-                    for (int k = 0; k < PIECE; ++k) o[k] *= inv;
+                    for (int k = 0; k < PIECE; k += 2) unpair(mul2(pair(o[k], o[k + 1]), pair(inv, inv)), o[k], o[k + 1]);
                     constexpr int N = 16 / sizeof(T);
 #pragma unroll
                     for (int p = 0; p < 8; ++p) {
@@ -543,7 +546,9 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, ChunkShape<T, D
             }
             // A weight of 0 does not hide an infinity or NaN among values that the row does not
             // see: rows that are not finite are computed again by a pass over what they see.
-            unsigned again = __ballot_sync(0xffffffffu, odd && live);
+            float n0, n1;
+            unpair(add2(naught[0], naught[1]), n0, n1);
+            unsigned again = __ballot_sync(0xffffffffu, live && !(n0 + n1 == 0.0f));
             while (again) {  // warp-uniform
                 const int src = __ffs((int)again) - 1;
                 again &= again - 1;
