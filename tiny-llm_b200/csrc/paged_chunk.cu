@@ -320,54 +320,74 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, ChunkShape<T, D
             {
                 const int g = lane >> 3, p = lane & 7;
                 uint8_t *const mine = sq + qt * QS * Sh::QBYTES + (warp & 3) * 32 * 128;
+                auto row_of = [&](int i) { return qt * kRows + 32 * (warp & 3) + 4 * i + g; };
+                auto source = [&](int x) {
+                    const int tx = token_of(x);
+                    return (const T *)A.q + (long long)(q.q0 + tok0 + tx) * A.q_stride + (long long)(head * G + h0 + x - tx * gs) * D +
+                           p * (16 / (int)sizeof(T));
+                };
+                auto target = [&](int i, int h, int piece) {
+                    const int xw = 4 * i + g;
+                    return mine + h * QHALF + xw * 128 + ((piece ^ (xw & 7)) * 16);
+                };
+                // all the loads of a batch before its first store: one latency
                 if constexpr (QS == 1) {
-#pragma unroll 4
+                    uint4 v[8][D / 64];
+#pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        const int xw = 4 * i + g, x = qt * kRows + 32 * (warp & 3) + xw, tx = token_of(x);
-                        const T *src = (const T *)A.q + (long long)(q.q0 + tok0 + tx) * A.q_stride +
-                                       (long long)(head * G + h0 + x - tx * gs) * D + p * 8;
+                        const T *src = source(row_of(i));
 #pragma unroll
                         for (int h = 0; h < D / 64; ++h)
-                            *reinterpret_cast<uint4 *>(mine + h * QHALF + xw * 128 + ((p ^ (xw & 7)) * 16)) =
-                                x < rows ? *reinterpret_cast<const uint4 *>(src + h * 64) : make_uint4(0, 0, 0, 0);
+                            v[i][h] = row_of(i) < rows ? *reinterpret_cast<const uint4 *>(src + h * 64) : make_uint4(0, 0, 0, 0);
                     }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+#pragma unroll
+                        for (int h = 0; h < D / 64; ++h) *reinterpret_cast<uint4 *>(target(i, h, p)) = v[i][h];
                 } else {
+                    // a lane takes 4 dimensions of every 32: whole lines per load
+                    constexpr int B = 4, N = D / 32;
                     float scaled = 1.0f;  // this lane's row
-#pragma unroll 4
-                    for (int i = 0; i < 8; ++i) {
-                        const int xw = 4 * i + g, x = qt * kRows + 32 * (warp & 3) + xw, tx = token_of(x);
-                        const T *src = (const T *)A.q + (long long)(q.q0 + tok0 + tx) * A.q_stride +
-                                       (long long)(head * G + h0 + x - tx * gs) * D + p * 8;
-                        float4 v[D / 64][2];
-                        float most = 0.0f;
+#pragma unroll 1
+                    for (int i0 = 0; i0 < 8; i0 += B) {
+                        float4 v[B][N];
 #pragma unroll
-                        for (int h = 0; h < D / 64; ++h)
+                        for (int j = 0; j < B; ++j) {
+                            const T *src = source(row_of(i0 + j));
 #pragma unroll
-                            for (int e = 0; e < 2; ++e)
-                                v[h][e] = x < rows ? *reinterpret_cast<const float4 *>(src + h * 64 + e * 4) : make_float4(0, 0, 0, 0);
+                            for (int k = 0; k < N; ++k)
+                                v[j][k] = row_of(i0 + j) < rows ? *reinterpret_cast<const float4 *>(src + k * 32)
+                                                                : make_float4(0, 0, 0, 0);
+                        }
+                        float most[B];
 #pragma unroll
-                        for (int h = 0; h < D / 64; ++h)
+                        for (int j = 0; j < B; ++j) {
+                            most[j] = 0.0f;
 #pragma unroll
-                            for (int e = 0; e < 2; ++e)
-                                most = fmaxf(most, fmaxf(fmaxf(fabsf(v[h][e].x), fabsf(v[h][e].y)),
-                                                         fmaxf(fabsf(v[h][e].z), fabsf(v[h][e].w))));
+                            for (int k = 0; k < N; ++k)
+                                most[j] = fmaxf(most[j], fmaxf(fmaxf(fabsf(v[j][k].x), fabsf(v[j][k].y)),
+                                                               fmaxf(fabsf(v[j][k].z), fabsf(v[j][k].w))));
+                        }
 #pragma unroll
-                        for (int d = 1; d < 8; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-                        // the row's largest value goes to [2^13, 2^14)
-                        const int e = max(14, min(254, (int)(__float_as_uint(most) >> 23)));
-                        const float up = __uint_as_float((uint32_t)(254 + 13 - e) << 23);
-                        const float of_row = __shfl_sync(0xffffffffu, up, (lane & 3) * 8);  // of row 4 i + lane % 4
-                        scaled = (lane >> 2) == i ? of_row : scaled;
+                        for (int d = 1; d < 8; d <<= 1)
 #pragma unroll
-                        for (int h = 0; h < D / 64; ++h) {
-                            uint4 hi, lo;
-                            split2(v[h][0].x * up, v[h][0].y * up, hi.x, lo.x);
-                            split2(v[h][0].z * up, v[h][0].w * up, hi.y, lo.y);
-                            split2(v[h][1].x * up, v[h][1].y * up, hi.z, lo.z);
-                            split2(v[h][1].z * up, v[h][1].w * up, hi.w, lo.w);
-                            uint8_t *dst = mine + h * QHALF + xw * 128 + ((p ^ (xw & 7)) * 16);
-                            *reinterpret_cast<uint4 *>(dst) = hi;
-                            *reinterpret_cast<uint4 *>(dst + Sh::QBYTES) = lo;
+                            for (int j = 0; j < B; ++j) most[j] = fmaxf(most[j], __shfl_xor_sync(0xffffffffu, most[j], d));
+#pragma unroll
+                        for (int j = 0; j < B; ++j) {
+                            // the row's largest value goes to [2^13, 2^14)
+                            const int e = max(14, min(254, (int)(__float_as_uint(most[j]) >> 23)));
+                            const float up = __uint_as_float((uint32_t)(254 + 13 - e) << 23);
+                            const float of_row = __shfl_sync(0xffffffffu, up, (lane & 3) * 8);  // of row 4 i + lane % 4
+                            scaled = (lane >> 2) == i0 + j ? of_row : scaled;
+#pragma unroll
+                            for (int k = 0; k < N; ++k) {
+                                uint2 hi, lo;
+                                split2(v[j][k].x * up, v[j][k].y * up, hi.x, lo.x);
+                                split2(v[j][k].z * up, v[j][k].w * up, hi.y, lo.y);
+                                uint8_t *dst = target(i0 + j, k / 2, (k & 1) * 4 + p / 2) + (p & 1) * 8;
+                                *reinterpret_cast<uint2 *>(dst) = hi;
+                                *reinterpret_cast<uint2 *>(dst + Sh::QBYTES) = lo;
+                            }
                         }
                     }
                     c = c / scaled;
@@ -494,7 +514,7 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, ChunkShape<T, D
             // piece p of row x lies at p ^ (x & 7): no bank conflicts either way
             uint8_t *const turn = sq + qt * QS * Sh::QBYTES + (warp & 3) * 32 * 128;
             constexpr int PIECE = 128 / sizeof(T);  // elements of a row per round
-#pragma unroll
+#pragma unroll 1  // the code of a round is fetched once, which takes as long as running it
             for (int d = 0; d < D; d += PIECE) {
                 float o[PIECE];
 #pragma unroll
