@@ -382,6 +382,40 @@ def test_a_prompt_from_its_beginning(tq, kind, cache, D):
     check(c, tq)
 
 
+@pytest.mark.parametrize("new,total", [
+    ([0, 200, 0, 40], [0, 290, 12, 60]), ([170, 30], [120, 0]), ([200, 170], [100, 170]), ([641], [641]),
+    ([129], [1290]), ([65, 90, 1], [4000, 3333, 700])])
+@pytest.mark.parametrize("H,KVH", [(8, 2), (7, 1), (4, 4)])
+def test_one_query_tile_per_item(tq, new, total, H, KVH):
+    """fp32 over fp16 with head_dim 128 and a table of some thousand positions."""
+    c = Case(new, total, H, KVH, 128, 16, True, "f32", "f16", pad=3, seed=len(new) + H, room=4096)
+    first = check(c, tq).clone()
+    assert torch.equal(first[sum(new):], torch.full_like(first[sum(new):], 7.0))
+    assert torch.equal(c.attend(tq)[:sum(new)], first[:sum(new)])
+
+
+@pytest.mark.parametrize("what", [math.nan, math.inf, -1])
+def test_masked_places_with_one_query_tile_per_item(tq, what):
+    new, total, x = 150, 900, 810
+    c = Case([new], [total], 8, 2, 128, 16, True, "f32", "f16", seed=3, room=4096)
+    if what == -1:  # a bad page
+        c.table_cpu[0, x // 16] = -1
+        c.upload()
+        check(c, tq, drop={(0, y) for y in range(x // 16 * 16, x // 16 * 16 + 16)})
+        assert int(c.status) == tq.PAGED_BAD_PAGE
+        return
+    want, most, vmax = c.want()
+    p = int(c.table_cpu[0, x // 16])
+    c.kview[p, 0, x % 16, 5] = what
+    c.vview[p, 0, x % 16, 7] = what
+    c.upload()
+    got = c.attend(tq).double().cpu()
+    blind = x - (total - new)
+    near(got[:blind], want[:blind], c.tolerance(most, vmax))
+    near(got[:, 4 * 128:], want[:, 4 * 128:], c.tolerance(most, vmax))
+    assert not torch.isfinite(got[blind:, 7]).all()
+
+
 @pytest.mark.parametrize("kind,cache", SIXTEEN)
 def test_tcgen05_calls_repeat_and_follow_a_graph(tq, kind, cache):
     """Items split over CTAs and joined: bit for bit the same every time, whatever other call used

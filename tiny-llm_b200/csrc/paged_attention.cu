@@ -73,12 +73,13 @@ int launch_paged_attention(const PagedAttnArgs &a, cudaStream_t st) {
         // The tcgen05 kernel needs a 16-bit cache and pays from some work on: its items cost
         // about 10 us before their first result.  Work is rows x positions x head_dim, the
         // positions bounded by the page table (the lengths are known on the device only):
-        // 14 heads x 64 tokens over 564 positions (32 M) 15.1 us by mma.sync, 18.0 by tcgen05;
-        // 32 heads of 128, 64 tokens over 564 (148 M) 24.2 and 23.3; 256 over 256 (268 M) 18.2
-        // and 13.7.  Up to 16 rows of queries per KV head mma.sync reads no key twice.
+        // 14 heads x 64 tokens over 564 positions (32 M) 14.6 us by mma.sync, 17.1 by tcgen05; 32
+        // heads of 128, 64 tokens over 164 (43 M) 10.7 and 13.2, 128 over 128 (67 M) 10.0 and
+        // 10.6, 48 over 448 (88 M) 20.9 and 16.5, 64 over 564 (148 M) 24.0 and 19.0.  Up to 16
+        // rows of queries per KV head mma.sync reads no key twice.
         const long long rows = (long long)a.b.max_q_len * (a.n_heads / a.n_kv_heads);
         const double work = (double)a.b.n_tokens * a.n_heads * a.b.max_len * a.head_dim;
-        if (a.cache_type != TQB200_EL_F32 && rows > kDecodeRows && work > 150e6) return launch_paged_chunk(a, st);
+        if (a.cache_type != TQB200_EL_F32 && rows > kDecodeRows && work > 60e6) return launch_paged_chunk(a, st);
         return launch_paged_decode(a, st);
     }
     if (a.type == TQB200_EL_F32)

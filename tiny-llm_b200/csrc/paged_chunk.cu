@@ -31,15 +31,20 @@
 //    issued copies and products are waited for (bounded), TMEM is freed and the error stored.
 //
 // Measured on one B200 (device time): 2048 rows of 32 heads over 8 KV heads of 128 and 16384
-// bf16 positions (515 GFLOP) 495 to 550 us by the clock's state, 0.94 to 1.04 PFLOP/s; 512 rows
-// of 32 heads over 4 KV heads, fp32 over fp16, 22.0 us.  What it came from, at the first shape:
+// bf16 positions (515 GFLOP) 470 to 550 us by the clock's state, 0.94 to 1.09 PFLOP/s; 512 rows
+// of 32 heads over 4 KV heads, fp32 over fp16, 19.1 us.  What it came from, at the first shape:
 // 861 us with a thread's own descriptors for every MMA (96 to 130 clocks each to issue, against
 // 64 now), 720 with one score buffer of 128 keys, 640 with two of 64, 519 with tiles by TMA
 // instead of 16-byte copies (without any copies it took 529 then: the copies were the bound).
 // Taking a quarter of the exponentials to a polynomial on the FMA pipe, or letting the two
 // query tiles take turns at the exponential, changed nothing.  A tile of 64 keys takes about
 // 2400 clocks for both query tiles, of which the products need 1280; the softmax warps' own
-// chain (TMEM load, maximum, exponential, TMEM store) is what is left.
+// chain (TMEM load, maximum, exponential, TMEM store) is what is left: with the weights apart
+// from the scores, so that the next scores need not wait for P V, it took as long or longer.
+// By pages of 16 the same chunk takes 544 us, 641 when one warp issued all the copies; by pages
+// of 8 573, 848 then and 661 by 16-byte copies.  An item's beginning and end (12000 of 29000
+// clocks for the 512 rows) run once, and their instructions' way to the SM counts: with the
+// results' loop unrolled the end alone took 6700 clocks, 2600 now.
 #include <cuda.h>
 #include <string.h>
 
@@ -211,19 +216,17 @@ struct ChunkShape {
     static constexpr int QS = std::is_same<T, float>::value ? 2 : 1;
     static constexpr int SOFT = QT * 128;                       // softmax threads
     static constexpr int FETCH = 2 * QT;                        // warps that fetch
-    static constexpr int THREADS = SOFT + FETCH * 32 + QT * 32;  // 14 warps per SM: 128 registers a thread
+    static constexpr int THREADS = SOFT + FETCH * 32 + QT * 32;  // QT 2: 14 warps, 128 registers a thread
     static constexpr int ROWS = QT * kRows;
     static constexpr uint32_t QBYTES = kRows * D * 2;           // one operand of one query tile
     static constexpr uint32_t TBYTES = KT * D * 2;              // one slot: a K or a V tile
     static constexpr uint32_t COLS = QT * (2 * KT + D) <= 256 ? 256 : 512;  // TMEM columns
-    // per SM: two where the queries leave room for it
-    static constexpr int CTAS = QT == 1 && QS * QBYTES <= 32768 ? 2 : 1;
     static_assert(QT * (2 * KT + D) <= 512, "TMEM");
 };
 
 // ---------------------------------------------------------------- the kernel
 template <typename T, typename C, int D, int QT>
-__global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, ChunkShape<T, D, QT>::CTAS)
+__global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, 1)
     paged_chunk_kernel(const __grid_constant__ ChunkParams P) {
     using Sh = ChunkShape<T, D, QT>;
     constexpr int QS = Sh::QS, ROWS = Sh::ROWS;
@@ -658,9 +661,9 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, ChunkShape<T, D
         // ================================================================ keys and values
         const int fw = warp - 4 * QT;
         // A tile whose positions all exist comes by tensor copies, one box of 64 dimensions of a
-        // page's slots (or 64 of them) per copy, each completing on the slot's barrier.  The
-        // others (a sequence's end, where what lies behind it must read as zeros; pages that do
-        // not divide a tile; bad pages) come by 16-byte copies, a row's 8 pieces by 8 lanes.
+        // page's slots (as many as divide a tile) per copy, each completing on the slot's barrier.
+        // The others (a sequence's end, where what lies behind it must read as zeros; pages that
+        // are not groups of 8 slots; bad pages) come by 16-byte copies, a row's 8 pieces by 8 lanes.
         constexpr int MINE = KT / Sh::FETCH;        // positions per warp: rows fw MINE + lane / 8 + 4 i
         constexpr int GRP = MINE / 4;
         const uint32_t ring0 = smem_u32(ring);
@@ -909,7 +912,7 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, ChunkShape<T, D
     if (tid == 0 && s_err) report(A.status, TQB200_PAGED_TIMEOUT);
 }
 
-// Two parts for each of the grid's CTAs, 256 rows of them per SM.
+// Two parts of up to 256 rows for each of the grid's CTAs, one per SM.
 size_t parts_floats(int head_dim) { return (size_t)std::min(4 * num_sms(), 2 * kSplitMaxCtas) * kRows * (size_t)(head_dim + 2); }
 
 // Tensor map over (dimension, slot, head, page) of one of the cache's arrays, boxes of 64
@@ -945,7 +948,6 @@ int launch_chunk_t(const PagedAttnArgs &a, cudaStream_t st) {
     static KernelSmem once;
     int limit = 0;
     TQ_CUDA_TRY(smem_limit_once(k, once, &limit));
-    if (Sh::CTAS == 2) limit = std::min(limit, 112 * 1024);  // of the SM's 228 KB, 1 KB per CTA reserved
     const int fixed = kMeta + QT * Sh::QS * (int)Sh::QBYTES;
     const int slots = std::min(kMaxSlots, (limit - fixed) / (int)Sh::TBYTES);
     TQ_CHECK_ARG(slots >= kBehind + 1, "paged_attention: %d bytes of shared memory hold %d tiles", limit, slots);
@@ -966,7 +968,7 @@ int launch_chunk_t(const PagedAttnArgs &a, cudaStream_t st) {
     }
     const long long items = (long long)P.line.heads * (a.b.n_seqs + (long long)a.b.n_tokens / P.line.tq);
     const long long most = items * ((std::max(1, a.b.max_len) + KT - 1) / KT);
-    const int grid = (int)std::min<long long>({(long long)num_sms() * Sh::CTAS, most, kSplitMaxCtas});
+    const int grid = (int)std::min<long long>({(long long)num_sms(), most, kSplitMaxCtas});
     k<<<grid, Sh::THREADS, fixed + slots * Sh::TBYTES, st>>>(P);
     TQ_CUDA_TRY(cudaGetLastError());
     return TQB200_OK;
@@ -974,13 +976,19 @@ int launch_chunk_t(const PagedAttnArgs &a, cudaStream_t st) {
 
 template <typename T, typename C>
 int launch_chunk_c(const PagedAttnArgs &a, cudaStream_t st) {
-    // One query tile per item where blocks of 256 rows would leave SMs idle and the pages can
-    // hold little more than the chunk (a prompt's beginning): 512 tokens of 32 heads 23.8 us
-    // against 28.9.  Over longer contexts two tiles per item, which halve the reads of the
-    // cache: 8 sequences of up to 509 tokens over up to 4600 positions 42.6 us against 67.
-    const bool big = (long long)a.b.n_tokens * a.n_heads >= 256LL * num_sms() || a.b.max_len > 2LL * a.b.max_q_len + KT;
-    if (a.head_dim == 64) return big ? launch_chunk_t<T, C, 64, 2>(a, st) : launch_chunk_t<T, C, 64, 1>(a, st);
-    return big ? launch_chunk_t<T, C, 128, 2>(a, st) : launch_chunk_t<T, C, 128, 1>(a, st);
+    // Two query tiles per item: they take turns at the tensor pipe and halve the reads of the
+    // cache.  The products of fp32 queries and weights (two operands each) of head_dim 128 keep the
+    // pipe so long that one tile per item, whose blocks of 128 rows reach more SMs, is quicker up to
+    // 5 G rows x positions x head_dim: 512 rows of 32 heads over 512 positions (1.1 G) 19.1 us
+    // against 24.2, 64 over 6064 (1.6 G) 46 and 60, 1000 over 1000 (4.1 G) 40.5 and 43.3; but 1200
+    // over 1200 (5.9 G) 63 and 60, 512 over 4512 (9.5 G) 115 and 91.  Elsewhere two are: 1500 bf16
+    // rows over 1500 48.0 us against 56.6, 1000 fp32 rows of head_dim 64 23.9 against 29.9.
+    if (a.head_dim == 64) return launch_chunk_t<T, C, 64, 2>(a, st);
+    if constexpr (std::is_same<T, float>::value) {
+        const double work = (double)a.b.n_tokens * a.n_heads * a.b.max_len * a.head_dim;
+        if (work < 5e9) return launch_chunk_t<T, C, 128, 1>(a, st);
+    }
+    return launch_chunk_t<T, C, 128, 2>(a, st);
 }
 
 }  // namespace
