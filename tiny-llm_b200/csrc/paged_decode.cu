@@ -495,17 +495,20 @@ __global__ void __launch_bounds__(kThreads, kPerSm<C, D, NB>) paged_decode_kerne
         if (__any_sync(0xffffffffu, bad_page) && lane == 0) report(A.status, TQB200_PAGED_BAD_PAGE);
 
         // ---- the warps' parts, joined through shared memory
-        // A weight of 0 does not hide an infinity or NaN.  Where some row of the item does not see
-        // some value, results that are not finite are computed again by a pass over what the row sees.
-        bool odd = false;
-        if (q.n > 1) {
+        // A weight of 0 does not hide an infinity or NaN among values that a row does not see, and the split
+        // of an operand makes a NaN of its own from an infinity (lo = 0 or of the other sign beside hi):
+        // results that are not finite are computed again by a pass over what the row sees.
+        uint64_t naught[2] = {pair(0.0f, 0.0f), pair(0.0f, 0.0f)};  // NaN once a value is not finite
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                for (int i = 0; i < MT; ++i)
+            for (int i = 0; i < MT; ++i)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) odd |= (__float_as_uint(o[nb][i][e]) & 0x7f800000u) == 0x7f800000u;
-        }
+                for (int e = 0; e < 4; e += 2)
+                    naught[e / 2] = fma2(pair(o[nb][i][e], o[nb][i][e + 1]), pair(0.0f, 0.0f), naught[e / 2]);
+        float n0, n1;
+        unpair(add2(naught[0], naught[1]), n0, n1);
+        const bool odd = !(n0 + n1 == 0.0f);
         const bool slow = __syncthreads_or(odd);  // also: every warp is done with the query operands
         if (slow) {
             for (int r = warp; r < ROWS; r += kWarps) {
