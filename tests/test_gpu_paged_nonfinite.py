@@ -97,3 +97,60 @@ def test_a_nan_key_spoils_its_own_heads(tq, kind, cache, new, total, room, D):
     r, blind = rows_of(c, seq), max(0, total[seq] // 2 - (total[seq] - new[seq]))
     want[r][:blind] = clean[r][:blind]
     same(c.attend(tq), want, c.tolerance(most, vmax))
+
+
+@pytest.mark.parametrize("kind,cache", [("bf16", "bf16"), ("f32", "f16")])
+def test_rows_computed_again_for_long_do_not_touch_other_sequences(tq, kind, cache):
+    """One sequence's infinity among 262 thousand positions.  Its 32 rows belong to one warp, whose passes
+    over what they see (0.2 us a position and row: 1.6 s) outlast the limit of the kernel's waits (2e9
+    clocks, 1.0 s), so they must not run beside them.  The rows of the sequences that the same
+    CTAs serve after it stay right, and nothing is reported.
+
+    Every sequence's page table names one page over and over (the first of sequence 0 its copy with the
+    infinity), so row i of n sees each of the page's positions N / P times, the last n - 1 - i of them
+    once less: the softmax of the page's scores with these counts.
+
+    Bound: N / 16 products in the tensor core, each cut by less than 2^-23 of the running sum, and
+    N / 64 fp32 additions of the weights' sum, beside what short contexts have."""
+    H, D, P, N, seqs = 16, 64, 64, 1 << 18, 200
+    new = [2] + [3] * (seqs - 1)
+    c = Case(new, [n + 61 for n in new], H, 1, D, P, True, kind, cache, seed=3, spare=0)
+    _, most, vmax = c.want()
+    c.pool = 2
+    g = torch.Generator().manual_seed(4)
+    c.k_cpu, c.v_cpu = (torch.randn(1, 1, P, D, generator=g).to(c.k_cpu.dtype).repeat(2, 1, 1, 1) for _ in range(2))
+    k, v = c.k_cpu[0, 0].double(), c.v_cpu[0, 0].double()
+    c.v_cpu[1, 0, 3, 7] = math.inf
+    c.table_cpu = torch.zeros(seqs, N // P, dtype=torch.int32)
+    c.table_cpu[0, 0] = 1
+    c.total = [N] * seqs
+    c.upload()
+    got = c.attend(tq).double().cpu()
+    torch.cuda.synchronize()
+    assert int(c.status) == 0
+    q = c.q_cpu[:, :H * D].double().view(c.n, H, D)
+    count = torch.full((c.n, P), float(N // P), dtype=torch.float64)
+    row = 0
+    for n in new:
+        for i in range(n):
+            count[row, P - (n - 1 - i):] -= 1
+            row += 1
+    s = torch.einsum("rhd,xd->rhx", q, k) * c.scale
+    w = (s - s.amax(-1, keepdim=True)).exp() * count[:, None]
+    want = torch.einsum("rhx,xd->rhd", w / w.sum(-1, keepdim=True), v).reshape(c.n, H * D)
+    want[:2].view(2, H, D)[..., 7] = math.inf
+    c.total = [P] * seqs  # the bound's terms of one page
+    same(got, want, c.tolerance(max(most, float(s.abs().max())), float(v.abs().max())) +
+         float(v.abs().max()) * (N / 16 * 2.0 ** -23 + N / 64 * 2.0 ** -24))
+
+
+def test_an_early_infinity_in_a_long_chunk(tq):
+    """Every row of a chunk sees it: element 7 is infinite, the others as without it."""
+    for kind, cache in (("bf16", "bf16"), ("f32", "f16")):
+        c = Case([256], [4096], 8, 2, 128, 16, True, kind, cache, seed=6, room=WIDE)
+        clean, most, vmax = c.want()
+        spoil(c, 0, 100, value=math.inf)
+        c.upload()
+        want = clean.clone()
+        want.view(256, 8, 128)[:, :4, 7] = math.inf
+        same(c.attend(tq), want, c.tolerance(most, vmax))

@@ -27,6 +27,7 @@
 //  * fp32 results: the tensor core cuts its sums, so after every 8 tiles O moves to an fp32 sum
 //    in the workspace and starts at zero (2000 rows over up to 8000 positions: 450 to 500 us by
 //    the clock's state, 430 without; error against 64 bits 2e-6 of the result instead of 6e-6).
+//  * Rows that come out not finite are computed again after the CTA's last item (redo_rows).
 //  * Every wait is bounded; after one runs out the roles go on without waiting or issuing, the
 //    issued copies and products are waited for (bounded), TMEM is freed and the error stored.
 //
@@ -224,6 +225,122 @@ struct ChunkShape {
     static_assert(QT * (2 * KT + D) <= 512, "TMEM");
 };
 
+// One row of an item from the parts of its CTAs, in order (thread = row).
+template <typename T, int D, int ROWS>
+__device__ __forceinline__ void join_row(const ChunkParams &P, const Line<KT> &it, int row, T *dst) {
+    const int c0 = it.first_cta(), c1 = it.last_cta();
+    auto part_of = [&](int cta) { return P.parts + it.slot_of(cta) * ROWS * (D + 2); };
+    // statistics, then 32 values at a time: two parts' loads in flight
+    float M = -INFINITY, L = 0.0f;
+#pragma unroll 4
+    for (int i = c0; i <= c1; ++i) M = fmaxf(M, __ldcg(part_of(i) + ROWS * D + row));
+    const float b = M == -INFINITY ? 0.0f : M;
+#pragma unroll 4
+    for (int i = c0; i <= c1; ++i) {
+        const float *pp = part_of(i) + ROWS * D + row;
+        L = fmaf(ex2(__ldcg(pp) - b), __ldcg(pp + ROWS), L);
+    }
+    const float li = L == 0.0f ? 0.0f : 1.0f / L;
+#pragma unroll 1
+    for (int d = 0; d < D; d += 32) {
+        float o[32];
+#pragma unroll
+        for (int k = 0; k < 32; ++k) o[k] = 0.0f;
+#pragma unroll 1
+        for (int i = c0; i <= c1; i += 2) {
+            const bool two = i < c1;
+            const float *p0 = part_of(i), *p1 = part_of(two ? i + 1 : i);
+            const float f0 = ex2(__ldcg(p0 + ROWS * D + row) - b);
+            const float f1 = two ? ex2(__ldcg(p1 + ROWS * D + row) - b) : 0.0f;
+            float4 x[8], y[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k] = __ldcg(reinterpret_cast<const float4 *>(p0 + ((d / 4 + k) * ROWS + row) * 4));
+#pragma unroll
+            for (int k = 0; k < 8; ++k) y[k] = __ldcg(reinterpret_cast<const float4 *>(p1 + ((d / 4 + k) * ROWS + row) * 4));
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                o[4 * k] = fmaf(f0, x[k].x, o[4 * k]), o[4 * k + 1] = fmaf(f0, x[k].y, o[4 * k + 1]);
+                o[4 * k + 2] = fmaf(f0, x[k].z, o[4 * k + 2]), o[4 * k + 3] = fmaf(f0, x[k].w, o[4 * k + 3]);
+            }
+            if (two) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    o[4 * k] = fmaf(f1, y[k].x, o[4 * k]), o[4 * k + 1] = fmaf(f1, y[k].y, o[4 * k + 1]);
+                    o[4 * k + 2] = fmaf(f1, y[k].z, o[4 * k + 2]), o[4 * k + 3] = fmaf(f1, y[k].w, o[4 * k + 3]);
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 32; ++k) o[k] *= li;
+#pragma unroll
+        for (int k = 0; k < 32; k += 16 / sizeof(T)) {
+            ElVec<T, 16 / sizeof(T)> v;
+            v.set(o + k);
+            v.store(dst + d + k);
+        }
+    }
+}
+
+// Whole CTA, after its last item: rows that came out not finite are computed again, each by a
+// warp's pass over what the row sees.  A weight of 0 does not hide an infinity or NaN among values
+// that the row does not see, and the split of an operand makes a NaN of its own from an infinity.
+// Such a pass takes 0.26 us a position (256 rows of 32 heads of 128 over 8192: 42 ms), which over
+// a long context outlasts the limits of the roles' waits; here nothing waits for it.  whole:
+// items that are this CTA's alone; later: its parts (bit: slot) whose tickets are still to be taken.
+template <typename T, typename C, int D, int QT>
+__device__ __noinline__ void redo_rows(const ChunkParams &P, bool whole, int later) {
+    using Sh = ChunkShape<T, D, QT>;
+    constexpr int ROWS = Sh::ROWS;
+    const PagedAttnArgs &A = P.A;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = A.n_heads / A.n_kv_heads;
+    __shared__ unsigned s_join;
+    Line<KT> it{};
+    it.template begin<Sh::THREADS>(A.b, P.line, nullptr);
+    for (; it.part(A.b); it.next(A.b)) {
+        const bool mine = it.all_mine();
+        const long long slot = it.slot_of(blockIdx.x);
+        if (mine ? !whole : !((later >> (slot & 1)) & 1)) continue;
+        const SeqInfo &q = it.q;
+        const int head = it.head / P.sets, h0 = (it.head - head * P.sets) * P.g_set;
+        const int gs = min(P.g_set, G - h0), tok0 = it.b * P.line.tq;
+        const int rows = min(P.line.tq, q.n - tok0) * gs;
+        auto at = [&](int row, long long stride) {
+            const int t = row / gs;
+            return (long long)(q.q0 + tok0 + t) * stride + (long long)(head * G + h0 + row - t * gs) * D;
+        };
+        float *part = P.parts + slot * ROWS * (D + 2);
+        for (int row = warp; row < rows; row += Sh::THREADS / 32) {
+            T *out = (T *)A.out + at(row, A.out_stride);
+            float naught = 0.0f;
+#pragma unroll
+            for (int e = lane; e < D; e += 32)
+                naught = fmaf(mine ? el_to_f<T>(out[e]) : part[(e / 4 * ROWS + row) * 4 + (e & 3)], 0.0f, naught);
+            if (!__any_sync(0xffffffffu, naught != 0.0f)) continue;  // NaN is not 0 either
+            float m, l, o[8];
+            row_pass<T, C>(A, (const T *)A.q + at(row, A.q_stride), it.seq, head, it.ta * KT,
+                           min(it.tb * KT, q.len - q.n + tok0 + row / gs + 1), m, l, o);
+            const float f = mine ? (l == 0.0f ? 0.0f : 1.0f / l) : exp2f(kLift);
+#pragma unroll
+            for (int j = 0; j < D / 32; ++j) {
+                const int e = lane + 32 * j;
+                if (mine) out[e] = el_from_f<T>(o[j] * f);
+                else part[(e / 4 * ROWS + row) * 4 + (e & 3)] = o[j] * f;
+            }
+            if (!mine && lane == 0) part[ROWS * D + row] = m, part[ROWS * D + ROWS + row] = l * f;
+        }
+        if (mine) continue;
+        __syncthreads();
+        const int c0 = it.first_cta();
+        if (tid == 0) {
+            s_join = take_ticket(&P.tickets[c0]) == (unsigned)(it.last_cta() - c0);
+            if (s_join) P.tickets[c0] = 0;
+        }
+        __syncthreads();
+        if (s_join && tid < rows) join_row<T, D, ROWS>(P, it, tid, (T *)A.out + at(tid, A.out_stride));
+        __syncthreads();  // s_join is read before it is written again
+    }
+}
+
 // ---------------------------------------------------------------- the kernel
 template <typename T, typename C, int D, int QT>
 __global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, 1)
@@ -246,7 +363,7 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, 1)
     static_assert(kMarks * KT / 8 <= kMeta - 512 && 8 * (2 * kMaxSlots + 8 * QT) + 4 <= 512, "meta");
     uint8_t *sq = smem + kMeta;
     uint8_t *ring = sq + QT * QS * Sh::QBYTES;
-    __shared__ int s_err;
+    __shared__ int s_err, s_odd, s_again, s_later;  // a part, a whole row is not finite; parts left to redo_rows
     __shared__ unsigned s_last;
 
     if (tid == 0) {
@@ -264,7 +381,7 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, 1)
             mbar_init(&done[i], 1);
         }
         fence_mbar_init();
-        s_err = 0;
+        s_err = s_odd = s_again = s_later = 0;
     }
     Line<KT> it{};
     it.template begin<Sh::THREADS>(A.b, P.line, A.status);
@@ -567,91 +684,23 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, 1)
                 part[ROWS * D + row] = m;
                 part[ROWS * D + ROWS + row] = l;
             }
-            // A weight of 0 does not hide an infinity or NaN among values that the row does not
-            // see: rows that are not finite are computed again by a pass over what they see.
+            // Rows that are not finite are computed again once the CTA's pipeline has ended (redo_rows): a
+            // part's ticket is left until then.
             float n0, n1;
             unpair(add2(naught[0], naught[1]), n0, n1);
-            unsigned again = __ballot_sync(0xffffffffu, live && !(n0 + n1 == 0.0f));
-            while (again) {  // warp-uniform
-                const int src = __ffs((int)again) - 1;
-                again &= again - 1;
-                const long long rr = __shfl_sync(0xffffffffu, q_row, src), hh = __shfl_sync(0xffffffffu, h_off, src);
-                const int ss = __shfl_sync(0xffffffffu, see, src), rw = __shfl_sync(0xffffffffu, row, src);
-                float mr, lr, orow[8];
-                row_pass<T, C>(A, (const T *)A.q + rr * A.q_stride + hh, it.seq, head, it.ta * KT, min(it.tb * KT, ss + 1), mr,
-                               lr, orow);
-                const float f = whole ? (lr == 0.0f ? 0.0f : 1.0f / lr) : exp2f(kLift);
-#pragma unroll
-                for (int j = 0; j < D / 32; ++j) {
-                    const int e = lane + 32 * j;
-                    if (whole) ((T *)A.out + rr * A.out_stride + hh)[e] = el_from_f<T>(orow[j] * f);
-                    else part[(e / 4 * ROWS + rw) * 4 + (e & 3)] = orow[j] * f;
-                }
-                if (!whole && lane == 0) {
-                    part[ROWS * D + rw] = mr;
-                    part[ROWS * D + ROWS + rw] = lr * f;
-                }
-            }
+            if (__any_sync(0xffffffffu, live && !(n0 + n1 == 0.0f)) && lane == 0) *(whole ? &s_again : &s_odd) = 1;
             if (!whole) {
                 // ---- the last of the item's CTAs joins the parts, in order
                 const int c0 = it.first_cta(), c1 = it.last_cta();
                 asm volatile("bar.sync 1, %0;" ::"n"(Sh::SOFT) : "memory");
-                if (tid == 0) s_last = take_ticket(&P.tickets[c0]) == (unsigned)(c1 - c0);
+                if (tid == 0) {
+                    if (s_odd) s_odd = 0, s_last = 0, s_later |= 1 << (it.slot_of(blockIdx.x) & 1);
+                    else s_last = take_ticket(&P.tickets[c0]) == (unsigned)(c1 - c0);
+                }
                 asm volatile("bar.sync 1, %0;" ::"n"(Sh::SOFT) : "memory");
                 if (s_last) {
                     if (tid == 0) P.tickets[c0] = 0;
-                    auto part_of = [&](int cta) { return P.parts + it.slot_of(cta) * ROWS * (D + 2); };
-                    if (live) {
-                        // statistics, then 32 values at a time: two parts' loads in flight
-                        float M = -INFINITY, L = 0.0f;
-#pragma unroll 4
-                        for (int i = c0; i <= c1; ++i) M = fmaxf(M, __ldcg(part_of(i) + ROWS * D + row));
-                        const float b = M == -INFINITY ? 0.0f : M;
-#pragma unroll 4
-                        for (int i = c0; i <= c1; ++i) {
-                            const float *pp = part_of(i) + ROWS * D + row;
-                            L = fmaf(ex2(__ldcg(pp) - b), __ldcg(pp + ROWS), L);
-                        }
-                        const float li = L == 0.0f ? 0.0f : 1.0f / L;
-#pragma unroll 1
-                        for (int d = 0; d < D; d += 32) {
-                            float o[32];
-#pragma unroll
-                            for (int k = 0; k < 32; ++k) o[k] = 0.0f;
-#pragma unroll 1
-                            for (int i = c0; i <= c1; i += 2) {
-                                const bool two = i < c1;
-                                const float *p0 = part_of(i), *p1 = part_of(two ? i + 1 : i);
-                                const float f0 = ex2(__ldcg(p0 + ROWS * D + row) - b);
-                                const float f1 = two ? ex2(__ldcg(p1 + ROWS * D + row) - b) : 0.0f;
-                                float4 x[8], y[8];
-#pragma unroll
-                                for (int k = 0; k < 8; ++k) x[k] = __ldcg(reinterpret_cast<const float4 *>(p0 + ((d / 4 + k) * ROWS + row) * 4));
-#pragma unroll
-                                for (int k = 0; k < 8; ++k) y[k] = __ldcg(reinterpret_cast<const float4 *>(p1 + ((d / 4 + k) * ROWS + row) * 4));
-#pragma unroll
-                                for (int k = 0; k < 8; ++k) {
-                                    o[4 * k] = fmaf(f0, x[k].x, o[4 * k]), o[4 * k + 1] = fmaf(f0, x[k].y, o[4 * k + 1]);
-                                    o[4 * k + 2] = fmaf(f0, x[k].z, o[4 * k + 2]), o[4 * k + 3] = fmaf(f0, x[k].w, o[4 * k + 3]);
-                                }
-                                if (two) {
-#pragma unroll
-                                    for (int k = 0; k < 8; ++k) {
-                                        o[4 * k] = fmaf(f1, y[k].x, o[4 * k]), o[4 * k + 1] = fmaf(f1, y[k].y, o[4 * k + 1]);
-                                        o[4 * k + 2] = fmaf(f1, y[k].z, o[4 * k + 2]), o[4 * k + 3] = fmaf(f1, y[k].w, o[4 * k + 3]);
-                                    }
-                                }
-                            }
-#pragma unroll
-                            for (int k = 0; k < 32; ++k) o[k] *= li;
-#pragma unroll
-                            for (int k = 0; k < 32; k += 16 / sizeof(T)) {
-                                ElVec<T, 16 / sizeof(T)> v;
-                                v.set(o + k);
-                                v.store(dst + d + k);
-                            }
-                        }
-                    }
+                    if (live) join_row<T, D, ROWS>(P, it, row, dst);
                 }
                 // s_last is read by every thread before it is written again: the next write
                 // follows the next item's first bar.sync
@@ -910,6 +959,7 @@ __global__ void __launch_bounds__(ChunkShape<T, D, QT>::THREADS, 1)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Sh::COLS) : "memory");
     }
     if (tid == 0 && s_err) report(A.status, TQB200_PAGED_TIMEOUT);
+    if (s_again | s_later) redo_rows<T, C, D, QT>(P, s_again != 0, s_later);
 }
 
 // Two parts of up to 256 rows for each of the grid's CTAs, one per SM.
