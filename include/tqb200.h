@@ -252,8 +252,10 @@ typedef struct tqb200_paged_cache {
  * entries past the sequence's last page are never read.  Rows at and behind q_start[n_seqs]
  * (a padded batch) are left as they are.  A sequence whose numbers do not fit (q_start
  * decreasing or past n_tokens, more than max_q_len rows, kv_len negative or past
- * table_stride pages) is skipped and TQB200_PAGED_BAD_SEQ recorded; a page index outside
- * [0, n_pages) is neither read nor written, its positions count as masked, and
+ * table_stride pages) is skipped and TQB200_PAGED_BAD_SEQ recorded, with rows or without; the
+ * others are served all the same (but a row in two of them, or in one of them and behind
+ * q_start[n_seqs], as decreasing entries can place it, may hold anything).  A page index
+ * outside [0, n_pages) is neither read nor written, its positions count as masked, and
  * TQB200_PAGED_BAD_PAGE is recorded. */
 typedef struct tqb200_paged_batch {
     const int *q_start;     /* [n_seqs + 1], not decreasing */

@@ -179,11 +179,44 @@ __device__ __forceinline__ SeqInfo seq_info(const BatchView &b, int s) {
     return seq_check(b, b.q_start[s], b.q_start[s + 1], b.kv_len[s]);
 }
 
-// The sequence that holds row t: the last s with q_start[s] <= t (32 candidates at a time by
-// the whole warp; every index stays in [0, n_seqs) whatever the array holds).  The caller
-// checks that the row lies inside it.
-__device__ __forceinline__ int seq_of_row(const BatchView &b, int t) {
+__device__ __forceinline__ void report(int *status, int code) {
+    if (status) atomicExch(status, code);
+}
+
+// Reports sequences whose numbers do not fit; a whole CTA, which has nothing else to do.
+static __device__ __noinline__ void check_seqs(const BatchView &b, int *status) {
+    bool bad = false;
+#pragma unroll 4
+    for (int s = threadIdx.x; s < b.n_seqs; s += blockDim.x) bad |= !seq_info(b, s).ok;
+    if (bad) report(status, TQB200_PAGED_BAD_SEQ);
+}
+
+// The first sequence that fits and holds row t, -1: none; by the whole warp, 128 at a time.
+static __device__ __noinline__ int scan_for_row(const BatchView &b, int t) {
     const int lane = threadIdx.x & 31;
+    for (int s0 = 0; s0 < b.n_seqs; s0 += 128) {
+        unsigned in = 0;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int i = s0 + 32 * u + lane;
+            if (i < b.n_seqs && b.q_start[i] <= t && b.q_start[i + 1] > t) in |= 1u << u;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int i = s0 + 32 * u;
+            const unsigned m = __ballot_sync(0xffffffffu, ((in >> u) & 1u) && seq_info(b, i + lane).ok);
+            if (m) return i + __ffs((int)m) - 1;
+        }
+    }
+    return -1;
+}
+
+// The sequence that holds row t, by the whole warp; ok == 0: none (a row behind the last, or of a
+// sequence to be skipped).
+__device__ __forceinline__ SeqInfo seq_of_row(const BatchView &b, int t, int &s) {
+    const int lane = threadIdx.x & 31;
+    // the last s with q_start[s] <= t, 32 candidates at a time (every index stays in [0, n_seqs)
+    // whatever the array holds)
     int lo = 0, n = b.n_seqs;  // candidates lo .. lo + n - 1; lo itself always stands
     while (n > 1) {
         const int step = (n + 31) / 32;
@@ -194,11 +227,18 @@ __device__ __forceinline__ int seq_of_row(const BatchView &b, int t) {
         n = min(step, n - last * step);
         lo += last * step;
     }
-    return lo;
-}
-
-__device__ __forceinline__ void report(int *status, int code) {
-    if (status) atomicExch(status, code);
+    s = lo;
+    SeqInfo q = seq_info(b, s);
+    if (q.ok && t >= q.q0 && t - q.q0 < q.n) return q;
+    const bool behind = q.ok && t >= q.q0 && s == b.n_seqs - 1;
+    q.ok = 0;
+    if (!behind) {
+        // An entry that decreases led the search astray: the rows of the sequences that fit must not be
+        // lost with the one that does not, so all of them are looked at.
+        s = scan_for_row(b, t);
+        if (s >= 0) q = seq_info(b, s);
+    }
+    return q;
 }
 
 // ---------------------------------------------------------------- launch arguments
@@ -237,16 +277,20 @@ __device__ __forceinline__ float ex2(float x) {
 
 // One warp's pass over positions [x0, x1) for one row (its p >= x1 - 1): the running maximum
 // of the scaled scores (base 2), the sum and, in lane l, elements l, l + 32, ... of the
-// weighted values.  Every element type, head_dim up to 256 and alignment; positions on pages
-// outside the cache are passed over.
-template <typename T, typename C>
-__device__ __noinline__ void row_pass(const PagedAttnArgs &A, const T *q, int seq, int kv_head, int x0, int x1,
-                         float &m, float &l, float (&o)[8]) {
+// weighted values (E of them: head_dim at most 32 E).  Every element type and alignment;
+// positions on pages outside the cache are passed over.  The next position's loads go out
+// before the present one is used (0.42 us a position for head_dim 96, 0.52 without).
+template <typename T, typename C, int E>
+__device__ __forceinline__ void row_pass(const PagedAttnArgs &A, const T *q, int seq, int kv_head, int x0, int x1,
+                                         float &m, float &l, float (&o)[E]) {
     const int lane = threadIdx.x & 31, D = A.head_dim;
-    float qv[8];
+    const PagedView kv = A.kv;
+    float qv[E];
+    int e[E];  // lanes past the end read its last element, so that no load hangs on a condition
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        qv[j] = lane + 32 * j < D ? el_to_f<T>(q[lane + 32 * j]) : 0.0f;
+    for (int j = 0; j < E; ++j) {
+        e[j] = min(lane + 32 * j, D - 1);
+        qv[j] = lane + 32 * j < D ? el_to_f<T>(q[e[j]]) : 0.0f;
         o[j] = 0.0f;
     }
     m = -INFINITY;
@@ -254,25 +298,35 @@ __device__ __noinline__ void row_pass(const PagedAttnArgs &A, const T *q, int se
     const float c = A.scale * kLog2e;
     const int *row = A.b.table + (long long)seq * A.b.table_stride;
     int bad = 0;
+    C kr[E], vr[E], kn[E], vn[E];
+    // position x's key and value, or (none, a bad page) the cache's first; its place, -1: none
+    auto load = [&](int x, C (&k)[E], C (&v)[E]) {
+        const long long at = x < x1 ? kv.offset(row, x, kv_head, &bad) : -1;
+        const C *kp = (const C *)kv.k + max(at, 0LL), *vp = (const C *)kv.v + max(at, 0LL);
+#pragma unroll
+        for (int j = 0; j < E; ++j) k[j] = kp[e[j]], v[j] = vp[e[j]];
+        return at;
+    };
+    long long at = load(x0, kr, vr);
+#pragma unroll 2  // the copies from next to present go
     for (int x = x0; x < x1; ++x) {
-        const long long at = A.kv.offset(row, x, kv_head, &bad);
-        if (at < 0) continue;  // warp-uniform
-        const C *k = (const C *)A.kv.k + at, *v = (const C *)A.kv.v + at;
-        float s = 0.0f, vv[8];
+        const long long next = load(x + 1, kn, vn);
+        if (at >= 0) {  // warp-uniform
+            float s = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const bool in = lane + 32 * j < D;
-            s = fmaf(qv[j], in ? el_to_f<C>(k[lane + 32 * j]) : 0.0f, s);
-            vv[j] = in ? el_to_f<C>(v[lane + 32 * j]) : 0.0f;
+            for (int j = 0; j < E; ++j) s = fmaf(qv[j], lane + 32 * j < D ? el_to_f<C>(kr[j]) : 0.0f, s);
+            s = warp_sum(s) * c;
+            const float mn = fmaxf(m, s);
+            const float base = mn == -INFINITY ? 0.0f : mn;
+            const float f = exp2f(m - base), p = exp2f(s - base);
+            m = mn;
+            l = fmaf(l, f, p);
+#pragma unroll
+            for (int j = 0; j < E; ++j) o[j] = fmaf(o[j], f, p * el_to_f<C>(vr[j]));
         }
-        s = warp_sum(s) * c;
-        const float mn = fmaxf(m, s);
-        const float base = mn == -INFINITY ? 0.0f : mn;
-        const float f = exp2f(m - base), p = exp2f(s - base);
-        m = mn;
-        l = fmaf(l, f, p);
+        at = next;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = fmaf(o[j], f, p * vv[j]);
+        for (int j = 0; j < E; ++j) kr[j] = kn[j], vr[j] = vn[j];
     }
     if (bad && lane == 0) report(A.status, TQB200_PAGED_BAD_PAGE);
 }

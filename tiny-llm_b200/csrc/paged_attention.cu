@@ -13,37 +13,36 @@ namespace {
 
 constexpr int kAnyThreads = 128;
 
-// One warp per (row, head).
-template <typename T, typename C>
+// One warp per (row, head), head_dim at most 32 E; with a status word one more CTA checks the sequences.
+template <typename T, typename C, int E>
 __global__ void __launch_bounds__(kAnyThreads) paged_attn_any_kernel(const __grid_constant__ PagedAttnArgs A) {
     const long long gw = (long long)blockIdx.x * (kAnyThreads / 32) + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
     const long long tok_ll = gw / A.n_heads;
+    if (A.status && blockIdx.x == gridDim.x - 1) return check_seqs(A.b, A.status);
     if (tok_ll >= A.b.n_tokens) return;
     const int tok = (int)tok_ll, head = (int)(gw - tok_ll * A.n_heads);
-    const int s = seq_of_row(A.b, tok);
-    const SeqInfo q = seq_info(A.b, s);
-    if (!q.ok) {
-        if (lane == 0) report(A.status, TQB200_PAGED_BAD_SEQ);
-        return;
-    }
-    if (tok < q.q0 || tok >= q.q0 + q.n) return;
+    int s;
+    const SeqInfo q = seq_of_row(A.b, tok, s);
+    if (!q.ok) return;
     const int pos = q.len - q.n + (tok - q.q0);
-    float m, l, o[8];
-    row_pass<T, C>(A, (const T *)A.q + tok * A.q_stride + (long long)head * A.head_dim, s,
-                   head / (A.n_heads / A.n_kv_heads), 0, pos + 1, m, l, o);
+    float m, l, o[E];
+    row_pass<T, C, E>(A, (const T *)A.q + tok * A.q_stride + (long long)head * A.head_dim, s,
+                      head / (A.n_heads / A.n_kv_heads), 0, pos + 1, m, l, o);
     T *out = (T *)A.out + tok * A.out_stride + (long long)head * A.head_dim;
     const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
+    for (int j = 0; j < E; ++j)
         if (lane + 32 * j < A.head_dim) out[lane + 32 * j] = el_from_f<T>(o[j] * inv);
 }
 
 template <typename T, typename C>
 int launch_any(const PagedAttnArgs &a, cudaStream_t st) {
     const long long blocks = ((long long)a.b.n_tokens * a.n_heads + kAnyThreads / 32 - 1) / (kAnyThreads / 32);
-    TQ_CHECK_ARG(blocks < (1LL << 31), "paged_attention: %d tokens of %d heads", a.b.n_tokens, a.n_heads);
-    paged_attn_any_kernel<T, C><<<(unsigned)blocks, kAnyThreads, 0, st>>>(a);
+    TQ_CHECK_ARG(blocks < (1LL << 31) - 1, "paged_attention: %d tokens of %d heads", a.b.n_tokens, a.n_heads);
+    const unsigned grid = (unsigned)blocks + (a.status ? 1 : 0);
+    if (a.head_dim <= 128) paged_attn_any_kernel<T, C, 4><<<grid, kAnyThreads, 0, st>>>(a);
+    else paged_attn_any_kernel<T, C, 8><<<grid, kAnyThreads, 0, st>>>(a);
     TQ_CUDA_TRY(cudaGetLastError());
     return TQB200_OK;
 }

@@ -284,8 +284,8 @@ __device__ __forceinline__ void join_row(const ChunkParams &P, const Line<KT> &i
 // Whole CTA, after its last item: rows that came out not finite are computed again, each by a
 // warp's pass over what the row sees.  A weight of 0 does not hide an infinity or NaN among values
 // that the row does not see, and the split of an operand makes a NaN of its own from an infinity.
-// Such a pass takes 0.26 us a position (256 rows of 32 heads of 128 over 8192: 42 ms), which over
-// a long context outlasts the limits of the roles' waits; here nothing waits for it.  whole:
+// Such passes (256 rows of 32 heads of 128 over 8192: 15 ms) may over a long context outlast
+// the limits of the roles' waits; here nothing waits for them.  whole:
 // items that are this CTA's alone; later: its parts (bit: slot) whose tickets are still to be taken.
 template <typename T, typename C, int D, int QT>
 __device__ __noinline__ void redo_rows(const ChunkParams &P, bool whole, int later) {
@@ -316,9 +316,9 @@ __device__ __noinline__ void redo_rows(const ChunkParams &P, bool whole, int lat
             for (int e = lane; e < D; e += 32)
                 naught = fmaf(mine ? el_to_f<T>(out[e]) : part[(e / 4 * ROWS + row) * 4 + (e & 3)], 0.0f, naught);
             if (!__any_sync(0xffffffffu, naught != 0.0f)) continue;  // NaN is not 0 either
-            float m, l, o[8];
-            row_pass<T, C>(A, (const T *)A.q + at(row, A.q_stride), it.seq, head, it.ta * KT,
-                           min(it.tb * KT, q.len - q.n + tok0 + row / gs + 1), m, l, o);
+            float m, l, o[D / 32];
+            row_pass<T, C, D / 32>(A, (const T *)A.q + at(row, A.q_stride), it.seq, head, it.ta * KT,
+                                   min(it.tb * KT, q.len - q.n + tok0 + row / gs + 1), m, l, o);
             const float f = mine ? (l == 0.0f ? 0.0f : 1.0f / l) : exp2f(kLift);
 #pragma unroll
             for (int j = 0; j < D / 32; ++j) {

@@ -117,6 +117,13 @@ __device__ __forceinline__ uint4 ld16(const char *p) {  // read once
 }
 __device__ __forceinline__ uint32_t word(const uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
+// row_pass out of line: the kernel's registers are its own.
+template <typename T, typename C, int E>
+__device__ __noinline__ void row_again(const PagedAttnArgs &A, const T *q, int seq, int kv_head, int x0, int x1, float &m,
+                                       float &l, float (&o)[E]) {
+    row_pass<T, C, E>(A, q, seq, kv_head, x0, x1, m, l, o);
+}
+
 // ---------------------------------------------------------------- the kernel
 // T activations, C cache, D head_dim, NB blocks of 8 query rows.
 template <typename C, int D, int NB>
@@ -512,14 +519,14 @@ __global__ void __launch_bounds__(kThreads, kPerSm<C, D, NB>) paged_decode_kerne
         const bool slow = __syncthreads_or(odd);  // also: every warp is done with the query operands
         if (slow) {
             for (int r = warp; r < ROWS; r += kWarps) {
-                float mr = -INFINITY, lr = 0.0f, orow[8];
+                float mr = -INFINITY, lr = 0.0f, orow[D / 32];
                 if (r < rows) {
                     const int x1 = min(tb * kTile, p0 + token_of(r) + 1);
-                    row_pass<T, C>(A, row_q(r), it.seq, head, ta * kTile, x1, mr, lr, orow);
+                    row_again<T, C, D / 32>(A, row_q(r), it.seq, head, ta * kTile, x1, mr, lr, orow);
                     const float lift = exp2f(kLift);
                     lr *= lift;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) orow[j] *= lift;
+                    for (int j = 0; j < D / 32; ++j) orow[j] *= lift;
                 }
                 for (int w = 0; w < kWarps; ++w) {
                     if (lane == 0) s_m[w][r] = w ? -INFINITY : mr, s_l[w][r] = w ? 0.0f : lr;

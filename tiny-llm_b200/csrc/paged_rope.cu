@@ -42,6 +42,7 @@ struct RopeParams {
     int *status;
     int lane_bits;           // log2 of the lanes of a row
     int warps;               // parts that a token is cut into, a warp each
+    int blocks;              // CTAs that take tokens; append with a status word: one more checks the sequences
     double log2_step;        // log2(theta) / h: frequency i is 2^(-i log2_step)
     double ratio;            // 2^-log2_step
 };
@@ -58,10 +59,8 @@ struct Place {
         cache_pos = 0;
         if constexpr (APPEND) {
             if (!q.ok || tok < q.q0 || tok >= q.q0 + q.n) {
-                seq = seq_of_row(P.b, tok);
-                q = seq_info(P.b, seq);
-                if (!q.ok && (threadIdx.x & 31) == 0) report(P.status, TQB200_PAGED_BAD_SEQ);
-                live = q.ok && tok >= q.q0 && tok < q.q0 + q.n;
+                q = seq_of_row(P.b, tok, seq);
+                live = q.ok;
             }
             cache_pos = q.len - q.n + (tok - q.q0);
         }
@@ -79,8 +78,10 @@ __global__ void __launch_bounds__(kRopeThreads, kRopePerSm) rope_vec_kernel(cons
     const int lane = threadIdx.x & 31;
     // warp gw: part `part` of tokens tok, tok + step, ... (step: whole tokens at a time)
     const int part = (int)(gw % P.warps);
-    const long long step = (long long)gridDim.x * (kRopeThreads / 32) / P.warps;
+    const long long step = (long long)P.blocks * (kRopeThreads / 32) / P.warps;
     long long tok = gw / P.warps;
+    if constexpr (APPEND)
+        if (blockIdx.x == (unsigned)P.blocks) return check_seqs(P.b, P.status);
     if (tok >= step || tok >= a.n_tokens) return;  // warp-uniform; no CTA barrier below
 
     const int bits = LB >= 0 ? LB : P.lane_bits;
@@ -289,6 +290,8 @@ __global__ void __launch_bounds__(kRopeThreads) rope_any_kernel(const __grid_con
     const int lane = threadIdx.x & 31;
     const int rows = a.n_heads + (APPEND ? 2 : 1) * a.n_kv_heads;
     const long long tok_ll = gw / rows;
+    if constexpr (APPEND)
+        if (blockIdx.x == (unsigned)P.blocks) return check_seqs(P.b, P.status);
     if (tok_ll >= a.n_tokens) return;
     const int tok = (int)tok_ll, row = (int)(gw - tok_ll * rows);
     Place place;
@@ -370,6 +373,7 @@ int launch_rope_t(RopeParams &P, cudaStream_t st) {
         vec = vec && multiple((uintptr_t)P.kv.k | (uintptr_t)P.kv.v, 16) &&
               multiple((uintptr_t)(P.kv.page_stride | P.kv.head_stride | P.kv.slot_stride), VEC);
     constexpr int kWarps = kRopeThreads / 32;
+    const int check = APPEND && P.status ? 1 : 0;
     if (vec) {
         P.lane_bits = bits;
         const int rpi = 32 >> bits;
@@ -378,7 +382,7 @@ int launch_rope_t(RopeParams &P, cudaStream_t st) {
         // groups dealt out) so that few tokens still reach every warp, and so that the last
         // round is full: the cost of parts p is the rounds times a part's groups and its
         // set-up, worth about 3 of them.
-        const long long resident = (long long)kRopePerSm * num_sms() * kWarps;
+        const long long resident = ((long long)kRopePerSm * num_sms() - check) * kWarps;
         int parts = 1;
         double best = 0.0;
         for (int p = 1; p <= std::min(n_it, 64); ++p) {
@@ -388,16 +392,18 @@ int launch_rope_t(RopeParams &P, cudaStream_t st) {
             if (p >= 4 && (long long)a.n_tokens * p >= resident) break;
         }
         P.warps = parts;
-        const long long blocks = std::min(((long long)a.n_tokens * parts + kWarps - 1) / kWarps, resident / kWarps);
-        if (bits == 3) rope_vec_kernel<T, C, APPEND, 3><<<(unsigned)blocks, kRopeThreads, 0, st>>>(P);
-        else if (bits == 4) rope_vec_kernel<T, C, APPEND, 4><<<(unsigned)blocks, kRopeThreads, 0, st>>>(P);
-        else if (bits == 5) rope_vec_kernel<T, C, APPEND, 5><<<(unsigned)blocks, kRopeThreads, 0, st>>>(P);
-        else rope_vec_kernel<T, C, APPEND, -1><<<(unsigned)blocks, kRopeThreads, 0, st>>>(P);
+        P.blocks = (int)std::min(((long long)a.n_tokens * parts + kWarps - 1) / kWarps, resident / kWarps);
+        const unsigned grid = P.blocks + check;
+        if (bits == 3) rope_vec_kernel<T, C, APPEND, 3><<<grid, kRopeThreads, 0, st>>>(P);
+        else if (bits == 4) rope_vec_kernel<T, C, APPEND, 4><<<grid, kRopeThreads, 0, st>>>(P);
+        else if (bits == 5) rope_vec_kernel<T, C, APPEND, 5><<<grid, kRopeThreads, 0, st>>>(P);
+        else rope_vec_kernel<T, C, APPEND, -1><<<grid, kRopeThreads, 0, st>>>(P);
     } else {
         const int rows = a.n_heads + (APPEND ? 2 : 1) * a.n_kv_heads;
         const long long blocks = ((long long)a.n_tokens * rows + kWarps - 1) / kWarps;
-        TQ_CHECK_ARG(blocks < (1LL << 31), "norm/rope: %d tokens of %d rows", a.n_tokens, rows);
-        rope_any_kernel<T, C, APPEND><<<(unsigned)blocks, kRopeThreads, 0, st>>>(P);
+        TQ_CHECK_ARG(blocks < (1LL << 31) - 1, "norm/rope: %d tokens of %d rows", a.n_tokens, rows);
+        P.blocks = (int)blocks;
+        rope_any_kernel<T, C, APPEND><<<(unsigned)blocks + check, kRopeThreads, 0, st>>>(P);
     }
     TQ_CUDA_TRY(cudaGetLastError());
     return TQB200_OK;
