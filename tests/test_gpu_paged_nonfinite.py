@@ -154,3 +154,42 @@ def test_an_early_infinity_in_a_long_chunk(tq):
         want = clean.clone()
         want.view(256, 8, 128)[:, :4, 7] = math.inf
         same(c.attend(tq), want, c.tolerance(most, vmax))
+
+
+@pytest.mark.parametrize("kind,cache", [("bf16", "bf16"), ("f16", "f16"), ("f32", "f16")])
+@pytest.mark.parametrize("D", [64, 128])
+def test_shared_items_computed_again_leave_the_workspace_ready(tq, kind, cache, D):
+    """Items that several CTAs share, some of whose parts come out not finite: their tickets are taken
+    late.  The call repeats bit for bit, in a graph too, and the next calls find the workspace ready."""
+    new, total, at = [90, 60, 17], [2500, 700, 3000], {0: 100, 2: 2990}
+    c = Case(new, total, 8, 2, D, 16, True, kind, cache, seed=8, room=WIDE)
+    h = c.handles(tq)
+    w = c.workspace(tq, *h)
+    first = c.attend(tq, work=w, handles=h).clone()
+    clean, most, vmax = c.want()
+    near(first, clean, c.tolerance(most, vmax))
+    finite = c.v.clone()
+    for seq, x in at.items():
+        spoil(c, seq, x, value=math.inf)
+    want = clean.clone()
+    for seq, x in at.items():
+        r = rows_of(c, seq)
+        blind = max(0, x - (total[seq] - new[seq]))
+        want[r][blind:].view(-1, 8, D)[:, :4, 7] = math.inf
+    c.v.copy_(c.v_cpu.to(c.v.device))
+    again = c.attend(tq, work=w, handles=h).clone()
+    same(again, want, c.tolerance(most, vmax))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        c.attend(tq, work=w, handles=h)
+    for _ in range(3):
+        c.obuf.fill_(7.0)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(c.out().view(torch.uint8), again.view(torch.uint8))
+    c.v.copy_(finite)
+    c.obuf.fill_(7.0)
+    assert torch.equal(c.attend(tq, work=w, handles=h), first)
+    assert int(c.status) == 0

@@ -138,3 +138,10 @@ def test_workspace_bytes():
     assert lib.paged_attention_workspace_bytes(cache(), batch(), 7) == 0  # refused by the call too
     small = lib.paged_attention_workspace_bytes(cache(), batch(), 8)
     assert lib.paged_attention_workspace_bytes(cache(), batch(n_seqs=500, n_tokens=500), 8) >= small
+
+
+def test_workspace_bytes_depend_on_head_dim_alone():
+    want = lib.paged_attention_workspace_bytes(cache(), batch(), 8)
+    for c, b, heads in ((cache(), batch(n_seqs=500, n_tokens=500, max_q_len=1), 8), (cache(n_pages=1 << 20), batch(), 32),
+                        (cache(type=lib.EL_F16, page_size=1, page_stride=128, head_stride=64, slot_stride=64), batch(), 2)):
+        assert lib.paged_attention_workspace_bytes(c, b, heads) == want
