@@ -193,3 +193,20 @@ def test_shared_items_computed_again_leave_the_workspace_ready(tq, kind, cache, 
     c.obuf.fill_(7.0)
     assert torch.equal(c.attend(tq, work=w, handles=h), first)
     assert int(c.status) == 0
+
+
+@pytest.mark.parametrize("seqs", [40, 500])
+@pytest.mark.parametrize("kind,cache", [("bf16", "bf16"), ("f32", "f16")])
+def test_rows_computed_again_among_many_sequences(tq, kind, cache, seqs):
+    """The second look finds its way through more sequences than a warp's lanes, than a CTA's threads."""
+    new = [0 if i % 7 == 3 else 5 for i in range(seqs)]
+    total = [n + 9 + (i * 37) % 120 for i, n in enumerate(new)]
+    c = Case(new, total, 8, 2, 64, 16, True, kind, cache, pad=1, seed=seqs, room=WIDE)
+    want, most, vmax = c.want()
+    for seq in (0, 2, seqs // 2, seqs - 1):
+        if new[seq]:
+            spoil(c, seq, 3, value=math.inf)
+            want[rows_of(c, seq)].view(-1, 8, 64)[:, :4, 7] = math.inf
+    c.upload()
+    same(c.attend(tq), want, c.tolerance(most, vmax))
+    assert int(c.status) == 0
