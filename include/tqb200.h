@@ -218,16 +218,21 @@ int tqb200_matvec_f16(const uint16_t *w, const float *x, float *y, int out_dim, 
  * No reference counterpart (the reference and tqb200_engine decode one request over one
  * contiguous cache).  For hosts that keep activations on the GPU and serve many sequences:
  * per layer, tqb200_dev_paged_append (query/key norms, RoPE, cache write) and then
- * tqb200_dev_paged_attention.  All pointers in this section are DEVICE pointers of the
- * current device (another device's, or a host pointer, is TQB200_ERR_INVALID_ARG); calls are
- * ordered on `stream`, allocate nothing, never synchronise, and may be captured in a CUDA
- * graph (sequence lengths and page tables are read on the device at every replay).
+ * tqb200_dev_paged_attention.  All pointers in this section are memory that the current
+ * device reads: its own, managed, or pinned host memory (another device's, or pageable host
+ * memory, is TQB200_ERR_INVALID_ARG); calls are ordered on `stream`, allocate nothing, never
+ * synchronise, and may be captured in a CUDA graph (sequence lengths and page tables are read
+ * on the device at every replay).
  *
  * Element types of activations (q, k, v, out) and of the cache.  The cache's type is the
  * activations' own, or TQB200_EL_F16 beside TQB200_EL_F32 activations; sums, norms and
- * softmax statistics are fp32 or wider, and results are rounded once, to nearest even
- * (fp16 subnormals kept: tqb200_engine's fp16 cache flushes |x| < 2^-24 as the reference
- * does). */
+ * softmax statistics are fp32 or wider, and results and what goes into the cache are rounded
+ * once, to nearest even (fp16 subnormals kept: tqb200_engine's fp16 cache flushes |x| < 2^-24
+ * as the reference does; an fp32 value past 65504 becomes an infinity in an fp16 cache).
+ * Attention with fp16 or bf16 activations and head_dim 64 or 128 also rounds each softmax
+ * weight to that type for its product with the values (the weights' sum stays fp32): 2.3e-3
+ * of the result in the 2-norm for bf16 and 2.8e-4 for fp16, where the result's own rounding
+ * makes 1.7e-3 and 2.1e-4. */
 enum { TQB200_EL_F32 = 0, TQB200_EL_F16 = 1, TQB200_EL_BF16 = 2 };
 
 /* One layer's cache: element (page p, KV head h, slot j, dimension d) of k and of v at
@@ -306,8 +311,11 @@ int tqb200_dev_paged_append(const void *q, const void *k, const void *v, void *q
 /* Causal attention of every sequence's new rows over its cached positions (the new rows'
  * own keys and values appended before):
  *   out[row, h] = sum_{x <= p} softmax_x(scale * q[row, h] . K[x, h / (n_heads / n_kv_heads)]) V[x, ...]
- * with p the row's position.  A row that sees no position (p < 0, or all its pages bad) gets
- * zeros.  out may not overlap q.  The workspace holds
+ * with p the row's position.  A row that sees no position (p < 0, or all its pages bad), or
+ * none with a score above -inf, gets zeros.  Infinities and NaN reach the rows that see them,
+ * as by the formula in fp32, and no others; rows that come out not finite are computed a
+ * second time, position by position, which costs some hundred times as long (256 rows of 32
+ * heads of 128 over 8192 positions: 15 ms).  out may not overlap q.  The workspace holds
  * tqb200_paged_attention_workspace_bytes() bytes, 16-byte aligned, zero before its first
  * call; every call leaves it ready for the next.  The bytes depend on the
  * device and head_dim alone, so one workspace serves chunks and single tokens, and any calls

@@ -160,7 +160,7 @@ struct PagedView {
 struct BatchView {
     const int *q_start, *kv_len, *table;
     int n_seqs, table_stride, n_tokens, max_q_len;
-    int max_len;  // table_stride * page_size (at most 2^31 - 1): the most positions
+    int max_len;  // table_stride * page_size (at most 0x7fff0000: a tile past it stays an int): the most positions
 };
 
 // A sequence's numbers, checked; ok == 0: to be skipped.
@@ -636,8 +636,7 @@ struct Line {
     }
 };
 
-// A driver function by name, looked up at run time (the library links no driver API); null
-// where there is none.
+// A driver function by name, looked up at run time; null where there is none.
 void *driver_entry(const char *name);
 int launch_qk_norm_rope(const RopeArgs &a, cudaStream_t st);
 int launch_paged_append(const RopeArgs &a, const PagedView &kv, int cache_type, const BatchView &b,
@@ -650,6 +649,6 @@ constexpr int kDecodeRows = 16;
 // The same with a 16-bit cache; blocks of 128 or 256 query rows.
 int launch_paged_chunk(const PagedAttnArgs &a, cudaStream_t st);
 size_t paged_chunk_work_bytes(int head_dim);
-size_t paged_attention_work_bytes(int n_heads, int n_kv_heads, int head_dim);
+size_t paged_attention_work_bytes(int head_dim);
 
 }  // namespace tqb200

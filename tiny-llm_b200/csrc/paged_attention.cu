@@ -60,8 +60,9 @@ void *driver_entry(const char *name) {
     return fn;
 }
 
-size_t paged_attention_work_bytes(int n_heads, int n_kv_heads, int head_dim) {
-    (void)n_heads, (void)n_kv_heads;
+// One size for chunks and single tokens, of any type: 59 MB for head_dim 128 on 148 SMs, most of it
+// the tcgen05 kernel's, so that a workspace made for one batch serves them all.
+size_t paged_attention_work_bytes(int head_dim) {
     return head_dim == 64 || head_dim == 128
                ? std::max(paged_decode_work_bytes(head_dim), paged_chunk_work_bytes(head_dim)) : 16;
 }
@@ -74,8 +75,10 @@ int launch_paged_attention(const PagedAttnArgs &a, cudaStream_t st) {
         // positions bounded by the page table (the lengths are known on the device only):
         // 14 heads x 64 tokens over 564 positions (32 M) 14.6 us by mma.sync, 17.1 by tcgen05; 32
         // heads of 128, 64 tokens over 164 (43 M) 10.7 and 13.2, 128 over 128 (67 M) 10.0 and
-        // 10.6, 48 over 448 (88 M) 20.9 and 16.5, 64 over 564 (148 M) 24.0 and 19.0.  Up to 16
-        // rows of queries per KV head mma.sync reads no key twice.
+        // 10.6, 48 over 448 (88 M) 20.9 and 16.5, 64 over 564 (148 M) 24.0 and 19.0, all with a page
+        // table as wide as the longest sequence.  With a wider one the small ones go to tcgen05 too: a table of
+        // 32768 positions costs the first 18.8 us against 15.9, the second 13.2 against 10.9.
+        // Up to 16 rows of queries per KV head mma.sync reads no key twice.
         const long long rows = (long long)a.b.max_q_len * (a.n_heads / a.n_kv_heads);
         const double work = (double)a.b.n_tokens * a.n_heads * a.b.max_len * a.head_dim;
         if (a.cache_type != TQB200_EL_F32 && rows > kDecodeRows && work > 60e6) return launch_paged_chunk(a, st);

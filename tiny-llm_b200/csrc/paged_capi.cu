@@ -267,7 +267,7 @@ size_t tqb200_paged_attention_workspace_bytes(const tqb200_paged_cache *cache,
         check_heads(op, n_heads, cache->n_kv_heads, cache->head_dim) || batch->n_seqs < 0 ||
         batch->n_seqs > (1 << 24) || batch->n_tokens < 0 || batch->max_q_len < 0)
         return 0;
-    return paged_attention_work_bytes(n_heads, cache->n_kv_heads, cache->head_dim);
+    return paged_attention_work_bytes(cache->head_dim);
 }
 
 int tqb200_dev_paged_attention(const void *q, void *out, int type, int n_heads, long long q_stride,

@@ -8,9 +8,10 @@
 //   O += P V (128 x D, fp32 in TMEM), P as the A operand from TMEM.
 // Bound: the tensor pipe for long chunks (4 D operations per row, key and value).  Beside it
 // runs one exponential per score on 16 lanes per clock, which takes as long as the products
-// of 16-bit operands (128 x 64 scores of D 128: 512 clocks either way), so two query tiles
-// alternate and each has two score buffers: the next tile's scores are formed while this one's
-// softmax runs.
+// of 16-bit operands at the pipe's rate (128 x 64 scores of D 128: 512 clocks either way), so two
+// query tiles alternate and each has two score buffers: the next tile's scores are formed while
+// this one's softmax runs.  As issued the products take 640 clocks: one of N = 64 (Q K^T) comes
+// every 48 clocks from its thread, where the pipe needs 32, one of N = 128 (P V) every 64.
 // Roles (warps): QT groups of 4 softmax warps (thread = query row = TMEM lane), 2 QT warps that
 // fetch keys and values, QT warps that each issue one query tile's products.
 //  * A ring of slots holds whole K or V tiles in the order they are used, K0 K1 V0 K2 V1 ...
@@ -21,7 +22,9 @@
 //    128-byte swizzle, as K-major A and B operands for Q K^T and MN-major B operand for P V.
 //  * Softmax: the row's maximum is raised only when a score passes it by 2^8 (then the warp
 //    rescales its rows of O in TMEM); weights carry a factor 2^6 against fp16's subnormals,
-//    so they stay below 2^14.
+//    so they stay below 2^14.  Of 16-bit activations they go into P V in the cache's type, off by
+//    at most half a step, their sum as it was: the chunk below comes out 2.3e-3 off 64 bits, 1.7e-3
+//    of it the results' own rounding; a second part for the weights would double P V.
 //  * fp32 activations over an fp16 cache: Q (scaled per row by a power of two) and P are
 //    split into fp16 hi + lo, two products each: 22 bits of either operand.
 //  * fp32 results: the tensor core cuts its sums, so after every 8 tiles O moves to an fp32 sum
@@ -33,19 +36,11 @@
 //
 // Measured on one B200 (device time): 2048 rows of 32 heads over 8 KV heads of 128 and 16384
 // bf16 positions (515 GFLOP) 470 to 550 us by the clock's state, 0.94 to 1.09 PFLOP/s; 512 rows
-// of 32 heads over 4 KV heads, fp32 over fp16, 19.1 us.  What it came from, at the first shape:
-// 861 us with a thread's own descriptors for every MMA (96 to 130 clocks each to issue, against
-// 64 now), 720 with one score buffer of 128 keys, 640 with two of 64, 519 with tiles by TMA
-// instead of 16-byte copies (without any copies it took 529 then: the copies were the bound).
-// Taking a quarter of the exponentials to a polynomial on the FMA pipe, or letting the two
-// query tiles take turns at the exponential, changed nothing.  A tile of 64 keys takes about
-// 2400 clocks for both query tiles, of which the products need 1280; the softmax warps' own
-// chain (TMEM load, maximum, exponential, TMEM store) is what is left: with the weights apart
-// from the scores, so that the next scores need not wait for P V, it took as long or longer.
-// By pages of 16 the same chunk takes 544 us, 641 when one warp issued all the copies; by pages
-// of 8 573, 848 then and 661 by 16-byte copies.  An item's beginning and end (12000 of 29000
-// clocks for the 512 rows) run once, and their instructions' way to the SM counts: with the
-// results' loop unrolled the end alone took 6700 clocks, 2600 now.
+// of 32 heads over 4 KV heads, fp32 over fp16, 19.3 us.  A tile of 64 keys takes about 2400 clocks
+// for both query tiles, of which the products as issued need 1280; the softmax warps' own chain
+// (TMEM load, maximum, exponential, TMEM store) is what is left.  Whole tiles by 16-byte copies take
+// 640 us at the first shape, by TMA 519; by pages of 16 it takes 544 us, by pages of 8 573.  An item's
+// beginning and end (12000 of 29000 clocks for the 512 rows) run once, so their code is kept short.
 #include <cuda.h>
 #include <string.h>
 
@@ -1032,7 +1027,9 @@ int launch_chunk_c(const PagedAttnArgs &a, cudaStream_t st) {
     // 5 G rows x positions x head_dim: 512 rows of 32 heads over 512 positions (1.1 G) 19.1 us
     // against 24.2, 64 over 6064 (1.6 G) 46 and 60, 1000 over 1000 (4.1 G) 40.5 and 43.3; but 1200
     // over 1200 (5.9 G) 63 and 60, 512 over 4512 (9.5 G) 115 and 91.  Elsewhere two are: 1500 bf16
-    // rows over 1500 48.0 us against 56.6, 1000 fp32 rows of head_dim 64 23.9 against 29.9.
+    // rows over 1500 48.0 us against 56.6, 1000 fp32 rows of head_dim 64 23.9 against 29.9.  (The
+    // positions are the page table's width, here that of the longest sequence; with a table of 32768
+    // the first takes two tiles and 24.8 us.)
     if (a.head_dim == 64) return launch_chunk_t<T, C, 64, 2>(a, st);
     if constexpr (std::is_same<T, float>::value) {
         const double work = (double)a.b.n_tokens * a.n_heads * a.b.max_len * a.head_dim;

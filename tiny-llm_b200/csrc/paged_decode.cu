@@ -22,7 +22,10 @@
 // Softmax: each warp keeps its own running maximum per row (shared by the warp's lanes),
 // raised only when a score passes it by 2^4 (one vote per 16 keys; else no shuffles), so
 // weights are at most 2^4; they carry a factor 2^6 that keeps small ones out of fp16's
-// subnormals.  Sums and accumulators are fp32.  The next 16 keys (and then values) are in
+// subnormals.  Sums and accumulators are fp32.  Of 16-bit activations a weight goes into P V in the
+// cache's type, off by at most half a step, its sum as it was: the results of 64 tokens over up
+// to 8192 bf16 positions are 2.0e-3 off 64 bits, 1.7e-3 of it their own rounding; a second part
+// for the weights would double the products.  The next 16 keys (and then values) are in
 // flight while the present ones are used; page numbers are read one step further ahead.
 //
 // Measured on one B200 (device time): 64 single tokens of 32 heads over 8 KV heads of 128, 126
